@@ -9,7 +9,8 @@ Four kinds of work:
 * ``pack``: an activation goes to 8 bits and comes back (row blocks).
 * ``gemm``: the product of two quantised matrices.  ``form`` "fwd": ``a[M, K] @ b[N, K].T``, "dgrad": ``a[M, K] @ b[K, N]``,
   "wgrad": ``a[K, M].T @ b[K, N]``.
-* ``linear``: one training step of a linear layer, forward and both gradients, the input kept in 8 bits in between.
+* ``linear``: one training step of a linear layer, forward and both gradients.  The forward product reads the input in row
+  blocks; what is kept of it for the weight's gradient are its tiles, in 8 bits too.
 * ``act``: silu (or silu(gate) * up) whose input is kept in 8 bits, and its gradient from what was kept.
 """
 from __future__ import annotations
@@ -223,7 +224,7 @@ def _plain(c, t):
         with torch.no_grad():
             x, w, dy = t
             xq, wq = _quantised(x, "row"), _quantised(w, "tile")
-            dw = _quantised(dy, "col").t() @ _quantised(xq, "tile")
+            dw = _quantised(dy, "col").t() @ _quantised(x, "tile")
             return (xq @ wq.t()).to(x.dtype), (_quantised(dy, "row") @ wq).to(x.dtype), dw.to(w.dtype)
     dt = t[0].dtype
     if c["gated"]:
@@ -318,8 +319,8 @@ def exact(case, seed):
         return torch.matmul(a.t() if form == "wgrad" else a, b.t() if form == "fwd" else b)
     if kind == "linear":
         x, w, dy = (v.double() for v in t)
-        x, w = _round8(x, "row"), _round8(w, "tile")
-        return (torch.matmul(x, w.t()), torch.matmul(_round8(dy, "row"), w),
+        w = _round8(w, "tile")
+        return (torch.matmul(_round8(x, "row"), w.t()), torch.matmul(_round8(dy, "row"), w),
                 torch.matmul(_round8(dy, "col").t(), _round8(x, "tile")))
     v = [u.double() for u in t]
     kept = [_round8(u, "row") for u in v[:-1]]
