@@ -44,7 +44,9 @@
 #include <string.h>
 
 #include "../device/prims.cuh"
+#include "../device/silu.cuh"
 #include "../device/tc_prims.cuh"
+#include "../device/tc_wait.cuh"
 #include "fused_schedule.h"
 #include "gemm_fused_parts.cuh"
 #include "gemm_tc.h"
@@ -91,23 +93,6 @@ static_assert(kThreads == fused::kGemmThreads, "comm and reducer code assumes th
 
 __device__ int g_pair_error;  // set when a wait of this kernel expired (read by mt_gemm_pair_error)
 
-__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatile int* abort_flag, uint64_t timeout_ns) {
-  uint32_t spins = 0;
-  uint64_t t0 = 0;
-  while (!mbar_try_wait(bar, parity)) {
-    if ((++spins & 0x3ffu) == 0) {
-      if (*abort_flag) return false;
-      const uint64_t now = globaltimer();
-      if (t0 == 0) t0 = now;
-      else if (now - t0 > timeout_ns) {
-        *abort_flag = 1;
-        return false;
-      }
-    }
-  }
-  return true;
-}
-
 // 32 bf16 of one row (64 bytes) in two 32-byte accesses, or in four of 16 bytes where the matrix is only aligned to that.
 __device__ __forceinline__ void store_row64(uint8_t* p, const uint32_t* v, bool wide) {
   if (wide) {
@@ -141,51 +126,6 @@ __device__ __forceinline__ void load_row64(const uint8_t* p, uint32_t* v, bool w
   }
 }
 
-// The same for a whole warp: one answer for all lanes, so that the issue loops stay warp-uniform.
-__device__ __noinline__ bool wait_bar_warp_slow(uint64_t* bar, uint32_t parity, volatile int* abort_flag, uint64_t timeout_ns) {
-  uint32_t spins = 0;
-  uint64_t t0 = 0;
-  while (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) {
-    if ((++spins & 0x3ffu) == 0) {
-      if (__any_sync(0xffffffffu, *abort_flag != 0)) return false;
-      const uint64_t now = __shfl_sync(0xffffffffu, globaltimer(), 0);
-      if (t0 == 0) t0 = now;
-      else if (now - t0 > timeout_ns) {
-        *abort_flag = 1;
-        return false;
-      }
-    }
-  }
-  return true;
-}
-__device__ __forceinline__ bool wait_bar_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag, uint64_t timeout_ns) {
-  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
-  return wait_bar_warp_slow(bar, parity, abort_flag, timeout_ns);
-}
-__device__ __forceinline__ bool aborted_warp(volatile int* abort_flag) { return __any_sync(0xffffffffu, *abort_flag != 0); }
-
-// silu and its derivative on packed bf16: the bits that x / (1 + exp(-x)) and sig * (1 + x * (1 - sig)) have as separate fp32
-// operations.  The quotients are Newton's iteration with Markstein's last correction (Computation of elementary functions on
-// the IBM RISC System/6000 processor, 1990) on y / 4, which keeps 4 / y a normal number up to the largest y: no branches, so
-// that the 32 elements of a step overlap.  CUDA's own quotient has a slow path for large y, which a lane in six takes where
-// h is spread over +- 64: silu in the epilogue of 8192 x 1792 x 4096 then took 205 us, 88.8 this way
-// (plain 83.0).  The fast exponential and quotient (87.3) are off by up to 1e-5 far from zero and flush silu to zero below
-// -87.3, where bf16 still has values.
-__device__ __forceinline__ float four_over(float y4) {   // 1 / y4 = 4 / y, y4 in [1 / 4, 2^126)
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(y4));
-  return __fmaf_rn(r, __fmaf_rn(-y4, r, 1.f), r);
-}
-__device__ __forceinline__ float silu1(float x) {
-  const float y = 1.f + expf(-x), y4 = 0.25f * y, x4 = 0.25f * x, r = four_over(y4), q0 = __fmul_rn(x4, r);
-  const float q = fabsf(q0) <= 3.4028234e38f ? __fmaf_rn(__fmaf_rn(-y4, q0, x4), r, q0) : q0;   // x infinite or NaN: as it is
-  return y <= 3.4028234e38f ? q : (y != y ? y : x * 0.f);                                       // y infinite: a zero
-}
-__device__ __forceinline__ float dsilu1(float d, float x) {
-  const float y = 1.f + expf(-x);
-  const float s = y <= 3.4028234e38f ? 0.25f * four_over(0.25f * y) : (y != y ? y : 0.f);
-  return __fmul_rn(d, __fmul_rn(s, __fadd_rn(1.f, __fmul_rn(x, 1.f - s))));
-}
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
   return *(uint32_t*)&p;
