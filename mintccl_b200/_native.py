@@ -139,6 +139,13 @@ def lib():
     sig("mt_mxfp8_reduce", i32, vp, vp, i32, u64, u64, u64, u64, pp, pp, u64, i32)
     sig("mt_mxfp8_quantize", i32, vp, i32, vp, vp, vp, u64)
     sig("mt_mxfp8_tile_scales", i32, vp, vp, vp, u64, u64)
+    i64 = C.c_int64
+    sig("mt_fp8_quantize", i32, vp, i32, vp, i64, i64, i64, i64, vp, vp, vp, vp, vp, vp)
+    sig("mt_fp8_dequantize", i32, vp, i32, vp, i64, vp, i64, i64, i64, i64, i32, i32, vp, i64)
+    sig("mt_fp8_act_forward", i32, vp, i32, vp, i64, vp, i64, i64, i64, vp, i64, i64, vp, vp, vp, vp)
+    sig("mt_fp8_act_backward", i32, vp, i32, i64, vp, vp, i64, i64, vp, vp, i64, i64, vp, i64, i64, i64, vp, vp, vp)
+    sig("mt_gemm_fp8", i32, vp, vp, i64, vp, i64, i64, vp, i64, vp, i64, i64, vp, i64, i32, i64, i64, i64, i32, i32, i32)
+    sig("mt_gemm_fp8_error", i32)
     sig("mt_test_wait_timeout", i32, vp, vp)
     sig("mt_test_one_rank_args", i32, u64, vp, u64, C.POINTER(u64))
     sig("mt_find_ring", i32, C.POINTER(C.c_double), i32, ip)

@@ -155,6 +155,32 @@ int mt_mxfp8_reduce(MtComm* c, void* stream, int op, uint64_t data_in_off, uint6
 int mt_mxfp8_quantize(void* stream, int dtype, const void* x, void* data, void* scale, uint64_t nelems);
 int mt_mxfp8_tile_scales(void* stream, const void* in, void* out, uint64_t rows, uint64_t kb);
 
+// ---- e4m3 with one fp32 scale per block of 128 (host/fp8_host.cu), on the current device -------------------------------
+// Payload rows are ldq bytes apart (a multiple of 16, at least cols; padding is written as zeros) and start on 16-byte
+// boundaries.  dtype: 0 fp32, 1 fp16, 2 bf16.  ld*: elements between rows.
+// Encodings of x [rows, cols]; any of the three may be null.  row_scale [ceil(cols / 128)][rows] (of blocks 1 x 128),
+// col_scale [ceil(rows / 128)][cols] (128 x 1), tile_scale [ceil(rows / 128)][ceil(cols / 128)].
+int mt_fp8_quantize(void* stream, int dtype, const void* x, int64_t ldx, int64_t rows, int64_t cols, int64_t ldq,
+                    void* row_data, void* row_scale, void* col_data, void* col_scale, void* tile_data, void* tile_scale);
+// out [rows, cols] = payload times scale, block (i, j)'s at scale[i * s_row + j * s_col]; row_block, col_block: 1 or 128.
+int mt_fp8_dequantize(void* stream, int dtype, const void* data, int64_t ldq, const void* scale, int64_t s_row, int64_t s_col,
+                      int64_t rows, int64_t cols, int row_block, int col_block, void* out, int64_t ldo);
+// y = silu(h) [* u], h [and u] encoded in row blocks (scales [ceil(cols / 128)][rows]).  u, u_data, u_scale: all null or none.
+int mt_fp8_act_forward(void* stream, int dtype, const void* h, int64_t ldh, const void* u, int64_t ldu, int64_t rows, int64_t cols,
+                       void* y, int64_t ldy, int64_t ldq, void* h_data, void* h_scale, void* u_data, void* u_scale);
+// dh [and du] from dy and what was kept; y (may be null): the activation again.  Outputs are contiguous.
+int mt_fp8_act_backward(void* stream, int dtype, int64_t ldq, const void* h_data, const void* h_scale, int64_t h_srow, int64_t h_scol,
+                        const void* u_data, const void* u_scale, int64_t u_srow, int64_t u_scol, const void* dy, int64_t lddy,
+                        int64_t rows, int64_t cols, void* dh, void* du, void* y);
+// C[M, N] (dtype) = sum over blocks kb of sa(m, kb) sb(n / 128, kb) A[m, kb] . B[n, kb].  A is stored [M, K], with ta [K, M];
+// B [N, K], with tb [K, N]; lda, ldb: bytes between stored rows (multiples of 16); sa(m, kb) = sa[m * sa_m + kb * sa_k],
+// likewise sb.  ta goes with tb.  nctas: 0, or at most this many CTAs.
+int mt_gemm_fp8(void* stream, const void* A, int64_t lda, const void* sa, int64_t sa_m, int64_t sa_k, const void* B, int64_t ldb,
+                const void* sb, int64_t sb_n, int64_t sb_k, void* C, int64_t ldc, int dtype, int64_t M, int64_t N, int64_t K,
+                int ta, int tb, int nctas);
+// 1 after a bounded wait of mt_gemm_fp8 expired (synchronises; the result of that call is then invalid), 0 otherwise
+int mt_gemm_fp8_error(void);
+
 // ---- device-wait self test: a wait nothing satisfies must time out and report, not hang -----------
 int mt_test_wait_timeout(MtComm* c, void* stream);
 // what the product of a one-rank plan is launched with (no GPU): out = {time limit in ns, status record, rank}

@@ -1,0 +1,179 @@
+"""e4m3 with a scale per block of 128, on the CPU: the encoding against its definition in 64 bits, the activations kept in 8
+bits against the formula and against differences, and what the entry points refuse."""
+import math
+
+import pytest
+import torch
+
+from mintccl_b200.ops import checkpoint8 as c8
+from mintccl_b200.ops import fp8
+
+BLOCKS = ["row", "col", "tile"]
+
+
+def values(shape, dtype, seed=0):
+    """Magnitudes over many powers of two, ties of e4m3, zero blocks, and values that are not finite."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(shape, generator=g, dtype=torch.float64)
+    top = {torch.float32: 120.0, torch.bfloat16: 120.0, torch.float16: 12.0}[dtype]
+    x = x * torch.exp2((torch.rand(shape[0], 1, generator=g, dtype=torch.float64) * 2 - 1) * top)
+    x = x.to(dtype)
+    flat = x.view(-1)
+    flat[::7] = 0.0
+    flat[3::11] = -0.0
+    if flat.numel() > 400:
+        flat[50] = float("inf")
+        flat[61] = float("-inf")
+        flat[72] = float("nan")
+        flat[300] = torch.finfo(dtype).max
+        flat[301] = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    return x
+
+
+def by_definition(x, block):
+    """Scales and values in 64 bits: a loop over blocks, the e4m3 values enumerated."""
+    codes = torch.arange(127, dtype=torch.float64)
+    ex, man = torch.div(codes, 8, rounding_mode="floor"), codes % 8
+    mags = torch.where(ex == 0, man / 512, (1 + man / 8) * torch.exp2(ex - 7))          # 0 ... 448, ascending
+    x = x.double()
+    br, bc = fp8.BLOCKS[block]
+    rows, cols = x.shape
+    want = torch.full_like(x, math.nan)
+    scales = torch.empty(-(-rows // br), -(-cols // bc), dtype=torch.float64)
+    for i in range(scales.shape[0]):
+        for j in range(scales.shape[1]):
+            b = x[i * br:(i + 1) * br, j * bc:(j + 1) * bc]
+            amax = b[b.isfinite()].abs().max().item() if b.isfinite().any() else 0.0
+            e = 0
+            if amax > 0:
+                e = math.frexp(amax)[1] - 9
+                e = max(-126, e if amax <= 448.0 * 2.0 ** e else e + 1)
+            s = scales[i, j] = 2.0 ** e
+            v = (b / s).abs()
+            at = torch.searchsorted(mags, v.contiguous()).clamp(max=126)
+            lo, hi = (at - 1).clamp(min=0), at
+            dl, dh = (v - mags[lo]).abs(), (v - mags[hi]).abs()
+            even = torch.where(lo % 2 == 0, lo, hi)
+            idx = torch.where(dl < dh, lo, torch.where(dh < dl, hi, even))
+            want[i * br:(i + 1) * br, j * bc:(j + 1) * bc] = torch.where(b.isfinite(), torch.sign(b) * mags[idx] * s, math.nan)
+    return scales, want
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("block", BLOCKS)
+@pytest.mark.parametrize("shape", [(1, 1), (1, 128), (3, 129), (128, 1), (129, 257), (260, 40)])
+def test_encoding_is_the_definition(shape, block, dtype):
+    x = values(shape, dtype)
+    data, scale = fp8.quantize_fp8(x, block)
+    want_scale, want = by_definition(x, block)
+    assert data.shape == x.shape and data.dtype is torch.uint8 and data.stride(0) % 16 == 0
+    assert torch.equal(scale.double(), want_scale)
+    got = data.view(torch.float8_e4m3fn).double() * fp8._spread(scale, *shape, block).double()
+    assert torch.equal(got.isnan(), want.isnan())
+    assert torch.equal(got.nan_to_num(), want.nan_to_num())
+    # restored in the tensor's own type: one rounding, and no infinity from a finite value
+    back = fp8.dequantize_fp8(data, scale, block, dtype)
+    top = torch.finfo(dtype).max
+    assert torch.equal(back.nan_to_num(nan=1.0), want.nan_to_num(nan=1.0).clamp(-top, top).to(dtype))
+
+
+def test_empty_tensors():
+    for shape in ((0, 5), (5, 0), (0, 0)):
+        for block in BLOCKS:
+            data, scale = fp8.quantize_fp8(torch.zeros(shape), block)
+            assert tuple(data.shape) == shape and tuple(scale.shape) == fp8._scale_shape(*shape, block)
+            assert tuple(fp8.dequantize_fp8(data, scale, block).shape) == shape
+
+
+@pytest.mark.parametrize("shape", [(), (1,), (300,), (2, 3, 130), (0, 4), (4, 0)])
+def test_saved_tensors_come_back(shape):
+    g = torch.Generator().manual_seed(1)
+    x = torch.randn(shape, generator=g).to(torch.bfloat16)
+    s = c8.save8(x)
+    y = s.restore()
+    assert y.shape == x.shape and y.dtype is x.dtype
+    # a rounding to e4m3 is half a step (2 ** -4 relative) of a normal value, 2 ** -10 times the scale below; the scale is
+    # at most 2 ** -7 of the largest magnitude
+    if x.numel():
+        assert bool(((y.double() - x.double()).abs() <= x.double().abs() * 2.0 ** -4 + x.double().abs().max() * 2.0 ** -17).all())
+    assert s.nbytes == x.numel() + 4 * s.scale.numel()
+    assert s.restore(torch.float32).dtype is torch.float32
+
+
+@pytest.mark.parametrize("gated", [False, True])
+def test_gradient_is_the_formulas_and_that_of_differences(gated):
+    g = torch.Generator().manual_seed(2)
+    h, u, dy = (torch.randn(4, 200, generator=g) for _ in range(3))
+    ins = [t.requires_grad_(True) for t in ((h, u) if gated else (h,))]
+    y = c8.swiglu8(*ins) if gated else c8.silu8(*ins)
+    hd, ud = h.detach().double(), u.detach().double() if gated else torch.ones(4, 200, dtype=torch.float64)
+    # 32 bits: a few roundings
+    torch.testing.assert_close(y.detach().double(), hd * torch.sigmoid(hd) * ud, rtol=2.0 ** -20, atol=2.0 ** -24)
+    y.backward(dy)
+    x = [c8.save8(t.detach()).restore().double().requires_grad_(True) for t in ins]
+    f = lambda a, b: a * torch.sigmoid(a) * b                                              # noqa: E731
+    ref = torch.autograd.grad(f(x[0], x[1] if gated else torch.ones_like(x[0])), x, dy.double())
+    for t, r in zip(ins, ref):
+        torch.testing.assert_close(t.grad.double(), r, rtol=2.0 ** -19, atol=2.0 ** -22)
+    # central differences in 64 bits at the kept values; the third derivative of silu is below 1: error step ** 2
+    step = 1e-4
+    b = x[1].detach() if gated else torch.ones(4, 200, dtype=torch.float64)
+    a = x[0].detach()
+    torch.testing.assert_close(ins[0].grad.double(), dy.double() * (f(a + step, b) - f(a - step, b)) / (2 * step), rtol=1e-5, atol=1e-6)
+
+
+def test_activation_at_the_ends_of_the_range():
+    h = torch.tensor([[-3e38, -200.0, -88.0, -0.0, 0.0, 88.0, 200.0, 3e38]])
+    y, saved = c8.silu8_forward(h)
+    assert torch.equal(y[0, [1, 3, 4, 6, 7]], torch.tensor([0.0, 0.0, 0.0, 200.0, 3e38]).where(torch.tensor([1, 0, 1, 1, 1]).bool(), torch.tensor(-0.0)))
+    d = c8.silu8_backward(saved, torch.ones_like(h))
+    assert d.isfinite().all() and d[0, -1] == 1 and d[0, 0] == 0
+
+
+def test_strided_and_expanded_gradients():
+    h = torch.randn(6, 150, requires_grad=True)
+    c8.silu8(h).sum().backward()
+    assert h.grad.shape == h.shape
+    both = torch.randn(2, 3, 260, requires_grad=True)
+    y = c8.swiglu8(both[..., :130], both[..., 130:])
+    y.transpose(0, 1).contiguous().sum().backward()
+    assert both.grad.isfinite().all() and y.shape == (2, 3, 130)
+
+
+def test_refusals():
+    x = torch.randn(4, 8)
+    for bad in (lambda: fp8.quantize_fp8(x, "rows"), lambda: fp8.quantize_fp8(x[0]), lambda: fp8.quantize_fp8(x.double()),
+                lambda: fp8.quantize_fp8_many(x, ()), lambda: fp8.quantize_fp8_many(x, ("row", "row")),
+                lambda: fp8.dequantize_fp8(*fp8.quantize_fp8(x), block="tiles"),
+                lambda: fp8.dequantize_fp8(*fp8.quantize_fp8(x), block="col"),
+                lambda: fp8.dequantize_fp8(*fp8.quantize_fp8(x), dtype=torch.float64),
+                lambda: fp8.dequantize_fp8(x, torch.ones(4, 1)),
+                lambda: c8.save8(x.long()), lambda: c8.silu8(x.int()), lambda: c8.swiglu8(x, x[:2]),
+                lambda: c8.swiglu8(x, x.half()), lambda: c8.silu8_backward(c8.save8(x), x[:2]),
+                lambda: c8.silu8_backward(c8.save8(x), x.half()),
+                lambda: fp8.gemm_fp8(*fp8.quantize_fp8(x), *fp8.quantize_fp8(x, "tile")),       # CPU tensors
+                lambda: fp8.gemm_fp8(*fp8.quantize_fp8(x), *fp8.quantize_fp8(x, "tile"), ta=True),
+                lambda: fp8.linear_fp8(x, x), lambda: fp8.linear_fp8(x, x[:, :4]), lambda: fp8.linear_fp8(x.double(), x.double())):
+        with pytest.raises(ValueError):
+            bad()
+
+
+def test_native_checks_come_before_any_launch():
+    """The C entry points refuse with an error code what a kernel could not run on; nothing here needs a GPU."""
+    from mintccl_b200 import _native as N
+    L = N.lib()
+    p = 1 << 20
+    assert L.mt_fp8_quantize(None, 0, p, 8, 0, 8, 16, p, p, None, None, None, None) < 0            # no rows
+    assert L.mt_fp8_quantize(None, 3, p, 8, 4, 8, 16, p, p, None, None, None, None) < 0            # type
+    assert L.mt_fp8_quantize(None, 0, p, 8, 4, 8, 24, p, p, None, None, None, None) < 0            # payload pitch
+    assert L.mt_fp8_quantize(None, 0, p, 8, 4, 8, 16, p + 8, p, None, None, None, None) < 0        # payload alignment
+    assert L.mt_fp8_quantize(None, 0, p, 8, 4, 8, 16, p, None, None, None, None, None) < 0         # no scales
+    assert L.mt_fp8_quantize(None, 0, p, 8, 4, 8, 16, None, None, None, None, None, None) < 0      # nothing wanted
+    assert L.mt_fp8_dequantize(None, 0, p, 16, p, 1, 1, 4, 8, 1, 64, p, 8) < 0                     # block size
+    assert L.mt_fp8_dequantize(None, 0, p, 16, p, 1, 1, 4, 8, 1, 128, p, 7) < 0                    # rows of out overlap
+    assert L.mt_fp8_act_forward(None, 0, p, 8, p, 8, 4, 8, p, 8, 16, p, p, None, None) < 0         # a gate without its copy
+    assert L.mt_fp8_act_backward(None, 0, 16, p, p, 1, 1, None, None, 0, 0, p, 8, 4, 8, p, p, None) < 0
+    ok = (None, p, 16, p, 1, 1, p, 16, p, 1, 1, p, 8, 0, 4, 8, 16, 0, 0, 0)
+    for i, v in ((1, None), (2, 8), (7, 0), (12, 7), (13, 5), (14, 0), (16, -1), (17, 1)):
+        assert L.mt_gemm_fp8(*ok[:i], v, *ok[i + 1:]) < 0, i
+    assert N.last_error()

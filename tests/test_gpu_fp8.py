@@ -1,0 +1,390 @@
+"""The kernels for e4m3 with a scale per block of 128: the encoding gives the bytes of the torch expressions (which the CPU
+tests hold to the definition), products and gradients are held to 64 bits."""
+import pytest
+import torch
+
+from mintccl_b200 import _native as N
+from mintccl_b200.ops import checkpoint8 as c8
+from mintccl_b200.ops import fp8
+from test_cpu_fp8 import values
+
+pytestmark = pytest.mark.gpu
+DTYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+def same_encoding(got, x, block):
+    want_data, want_scale = fp8._torch_quantize(x.cpu(), block)
+    assert torch.equal(got[1].cpu(), want_scale)
+    assert torch.equal(got[0].cpu(), want_data)
+
+
+# ---- encoding, decoding -----------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(1, 1), (1, 127), (1, 4096), (3, 129), (31, 256), (32, 128), (33, 1000), (128, 128), (129, 257),
+                                   (300, 640), (1000, 16)])
+def test_encoding_gives_the_bytes_of_the_torch_path(shape, dtype):
+    x = values(shape, dtype, seed=shape[1]).cuda()
+    for block in fp8.BLOCKS:
+        same_encoding(fp8.quantize_fp8(x, block), x, block)
+    for blocks in (("row", "col"), ("row", "tile"), ("tile", "col"), ("col", "row", "tile")):
+        for block, got in zip(blocks, fp8.quantize_fp8_many(x, blocks)):
+            same_encoding(got, x, block)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_encoding_takes_any_layout(dtype):
+    base = values((70, 700), dtype).cuda()
+    for x in (base[:, 1:600], base[:, 8:520], base[::2, 16:272], base.t(), base[:, ::3], base[:1].expand(40, 700), base[3:4, 5:],
+              base[:, 5:6]):
+        for block in fp8.BLOCKS:
+            same_encoding(fp8.quantize_fp8(x, block), x, block)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("block", list(fp8.BLOCKS))
+@pytest.mark.parametrize("shape", [(1, 1), (1, 300), (33, 1000), (129, 256), (256, 17)])
+def test_decoding_gives_the_values_of_the_torch_path(shape, block, dtype):
+    x = values(shape, dtype, seed=3)
+    data, scale = fp8.quantize_fp8(x, block)
+    want = fp8.dequantize_fp8(data, scale, block, dtype)
+    for d, s in ((data.cuda(), scale.cuda()),                                             # copies lose the padding
+                 fp8.quantize_fp8(x.cuda(), block),
+                 (data.cuda().view(torch.float8_e4m3fn), scale.cuda().t().contiguous().t())):
+        got = fp8.dequantize_fp8(d, s, block, dtype)
+        assert got.is_contiguous() and torch.equal(got.cpu().nan_to_num(nan=1.0), want.nan_to_num(nan=1.0))
+        assert torch.equal(got.cpu().isnan(), want.isnan())
+
+
+def test_a_long_tensor_and_a_long_row():
+    g = torch.Generator(device="cuda").manual_seed(0)
+    for shape in ((2_300_000_000 // 4096, 4096), (1, 70_000_001)):          # offsets past 31 bits; one row of many blocks
+        x = torch.randn(shape, generator=g, device="cuda", dtype=torch.bfloat16)
+        s = c8.save8(x)
+        last = (slice(-3, None), slice((shape[1] - 1) // 128 * 128 - 1024, None))        # whole blocks, then what is left
+        tail = x[last]
+        want = fp8._torch_quantize(tail, "row")
+        assert torch.equal(s.data[last], want[0])
+        assert torch.equal(s.restore()[last], fp8.dequantize_fp8(*want, "row", torch.bfloat16))
+        del x, s, tail
+
+
+# ---- products ----------------------------------------------------------------------------------------------------------
+def operands(form, M, N, K, seed=0, spread=1.0):
+    """Payloads and scales on the GPU, and the matrices they stand for in 64 bits."""
+    g = torch.Generator(device="cuda").manual_seed(seed + M + 3 * N + 5 * K)
+
+    def one(rows, cols, block):
+        data = fp8._new_payload(rows, cols, "cuda")
+        v = (torch.randn(rows, cols, generator=g, device="cuda") * 100).clamp(-448, 448)
+        data.copy_(v.to(torch.float8_e4m3fn).view(torch.uint8))
+        scale = fp8._new_scale(rows, cols, block, "cuda")
+        scale.copy_(torch.exp2((torch.rand(scale.shape, generator=g, device="cuda") * 2 - 1) * spread) * 0.01)
+        return data, scale, data.view(torch.float8_e4m3fn).double() * fp8._spread(scale, rows, cols, block).double()
+
+    a = one(K, M, "col") if form == "wgrad" else one(M, K, "row")
+    b = one(N, K, "tile") if form == "fwd" else one(K, N, "tile")
+    return a[:2], b[:2], a[2].t() if form == "wgrad" else a[2], b[2].t() if form == "fwd" else b[2]
+
+
+def product(form, a, b, **kw):
+    return fp8.gemm_fp8(*a, *b, ta=form == "wgrad", tb=form != "fwd", **kw)
+
+
+def check_product(got, a64, b64):
+    """Roundings to 32 bits: one for each block's scale product and one for each addition of a block, 2 ** -24 each; inside
+    a block four steps of 32 products, for which the tensor core keeps at least 24 bits below the largest (32 * 2 ** -27 at
+    the 27 bits measured, 4 * 2 ** -23 for the steps' own roundings): together (K / 128 + 16) * 2 ** -23 of the sum of
+    magnitudes.  Then one rounding to the output's type, or half of its smallest value."""
+    want, mag = a64 @ b64, a64.abs() @ b64.abs()
+    info = torch.finfo(got.dtype)
+    blocks = -(-a64.shape[1] // 128)
+    tol = mag * ((blocks + 16) * 2.0 ** -23) * (1 + info.eps) + want.abs() * info.eps / 2 + info.smallest_normal * info.eps
+    bad = ((got.double() - want).abs() > tol).nonzero()
+    assert not len(bad), (bad[:4].tolist(), len(bad))
+
+
+SIZES = [(1, 1, 1), (1, 128, 128), (3, 5, 7), (1, 4096, 4096), (17, 300, 129), (64, 1000, 512), (127, 129, 257), (128, 256, 384),
+         (130, 1000, 1111), (257, 515, 2050), (300, 127, 16), (2050, 1800, 260), (512, 4096, 1792), (129, 20000, 100)]
+
+
+@pytest.mark.parametrize("form", ["fwd", "dgrad", "wgrad"])
+@pytest.mark.parametrize("size", SIZES)
+def test_product_against_64_bits(size, form):
+    a, b, a64, b64 = operands(form, *size, spread=4.0)
+    for dtype in DTYPES:
+        check_product(product(form, a, b, dtype=dtype), a64, b64)
+    assert N.lib().mt_gemm_fp8_error() == 0
+
+
+@pytest.mark.parametrize("form", ["fwd", "dgrad", "wgrad"])
+def test_product_takes_any_layout(form):
+    M, Nn, K = 200, 333, 500
+    a, b, a64, b64 = operands(form, M, Nn, K)
+    wide = torch.zeros(M, 512, device="cuda", dtype=torch.float16)
+    for out in (wide[:, 8:8 + Nn], wide[:, 3:3 + Nn], wide[:, :Nn]):
+        wide.zero_()
+        got = product(form, a, b, out=out)
+        assert got is out
+        check_product(got, a64, b64)
+        assert int((wide != 0).sum()) == int((out != 0).sum())            # nothing beside the output is written
+    # tight rows (not on 16-byte boundaries), float8 views, transposed storage, scales in another order
+    tight = [(d.contiguous().view(torch.float8_e4m3fn), s.t().contiguous().t()) for d, s in (a, b)]
+    check_product(product(form, *tight), a64, b64)
+    turned = [(d.t().contiguous().t(), s.contiguous()) for d, s in (a, b)]
+    check_product(product(form, *turned, nctas=3), a64, b64)
+    assert torch.equal(product(form, *tight), product(form, a, b))
+
+
+def test_rows_behind_the_output_are_left_alone():
+    a, b, a64, b64 = operands("fwd", 100, 200, 300)
+    buf = torch.full((140, 208), 7.0, device="cuda", dtype=torch.bfloat16)
+    check_product(product("fwd", a, b, out=buf[20:120, :200]), a64, b64)
+    buf[20:120, :200] = 7.0
+    assert bool((buf == 7.0).all())
+
+
+def test_empty_products():
+    z = lambda *s: torch.zeros(s, device="cuda", dtype=torch.uint8)                                  # noqa: E731
+    f = lambda *s: torch.zeros(s, device="cuda")                                                     # noqa: E731
+    assert fp8.gemm_fp8(z(0, 64), f(0, 1), z(32, 64), f(1, 1)).shape == (0, 32)
+    got = fp8.gemm_fp8(z(0, 64), f(0, 64), z(0, 32), f(0, 1), ta=True, tb=True, out=torch.ones(64, 32, device="cuda"))
+    assert got.shape == (64, 32) and bool((got == 0).all())
+
+
+def test_values_that_are_not_finite_stay_in_their_rows():
+    a, b, a64, b64 = operands("fwd", 130, 260, 300)
+    a[0].view(torch.uint8)[5, 7] = 0x7f
+    a[1][9, 1] = float("inf")
+    got = product("fwd", a, b)
+    assert bool(got[5].isnan().all()) and not bool(got[9].isfinite().any())
+    keep = [i for i in range(130) if i not in (5, 9)]
+    check_product(got[keep], a64[keep], b64)
+
+
+def test_product_offsets_past_31_bits():
+    M, Nn, K = 70_016, 32_768 + 8, 128
+    a, b, a64, b64 = operands("fwd", M, Nn, K)
+    got = product("fwd", a, b)
+    rows = [0, 1, 65_535, 65_536, M - 1]
+    check_product(got[rows], a64[rows], b64)
+
+
+def test_product_gives_the_same_bits_again():
+    a, b, *_ = operands("fwd", 1000, 1111, 2050)
+    first = product("fwd", a, b, dtype=torch.float32)
+    for _ in range(5):
+        assert torch.equal(product("fwd", a, b, dtype=torch.float32), first)
+
+
+def test_products_on_two_streams_and_in_a_graph():
+    a, b, a64, b64 = operands("fwd", 300, 700, 900)
+    c, d, c64, d64 = operands("dgrad", 500, 600, 1000)
+    torch.cuda.synchronize()
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    outs = []
+    for _ in range(10):
+        with torch.cuda.stream(s1):
+            outs.append((product("fwd", a, b), a64, b64))
+        with torch.cuda.stream(s2):
+            outs.append((product("dgrad", c, d), c64, d64))
+    torch.cuda.synchronize()
+    for o in outs:
+        check_product(*o)
+    x = torch.randn(100, 384, device="cuda", dtype=torch.bfloat16)
+    w = fp8.quantize_fp8(torch.randn(256, 384, device="cuda"), "tile")
+    step = lambda t: fp8.gemm_fp8(*fp8.quantize_fp8(t), *w)                                          # noqa: E731
+    step(x)
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = step(x)
+        graphs.append((g, y))
+    x.copy_(torch.randn_like(x) * 3)
+    with torch.cuda.stream(s1):
+        s1.wait_stream(torch.cuda.default_stream())
+        graphs[0][0].replay()
+    with torch.cuda.stream(s2):
+        s2.wait_stream(torch.cuda.default_stream())
+        graphs[1][0].replay()
+    torch.cuda.synchronize()
+    assert torch.equal(graphs[0][1], step(x)) and torch.equal(graphs[1][1], step(x))
+
+
+def test_refusals_on_the_gpu():
+    x = torch.randn(64, 128, device="cuda")
+    a, sa = fp8.quantize_fp8(x)
+    b, sb = fp8.quantize_fp8(x, "tile")
+    for bad in (lambda: fp8.gemm_fp8(a, sb, b, sb), lambda: fp8.gemm_fp8(a, sa, b, sa), lambda: fp8.gemm_fp8(a, sa.double(), b, sb),
+                lambda: fp8.gemm_fp8(a, sa, b[:, :64], sb), lambda: fp8.gemm_fp8(x, sa, b, sb), lambda: fp8.gemm_fp8(a, sa, b, sb, ta=True),
+                lambda: fp8.gemm_fp8(a, sa, b, sb, dtype=torch.float64), lambda: fp8.gemm_fp8(a, sa.cpu(), b, sb),
+                lambda: fp8.gemm_fp8(a, sa, b, sb, out=torch.empty(64, 65, device="cuda")),
+                lambda: fp8.gemm_fp8(a, sa, b, sb, out=torch.empty(64, 64, device="cuda").t()),
+                lambda: fp8.gemm_fp8(a, sa, b, sb, out=torch.empty(64, 64)), lambda: fp8.dequantize_fp8(a, sa.cpu()),
+                lambda: fp8.linear_fp8(x, x.cpu()), lambda: fp8.linear_fp8(x, x, w_fp8=(b[:32], sb))):
+        with pytest.raises(ValueError):
+            bad()
+
+
+# ---- the linear layer ------------------------------------------------------------------------------------------------
+def trip(t, block):
+    return fp8.dequantize_fp8(*fp8.quantize_fp8(t.detach(), block), block).double()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lead,fin,fout", [((1,), 64, 64), ((2, 65), 300, 130), ((1000,), 512, 1000), ((3, 1, 7), 129, 257)])
+def test_linear_layer_and_its_gradients(lead, fin, fout, dtype):
+    g = torch.Generator(device="cuda").manual_seed(fin)
+    x = torch.randn(*lead, fin, generator=g, device="cuda").to(dtype).requires_grad_(True)
+    w = (torch.randn(fout, fin, generator=g, device="cuda") * 0.05).to(dtype).requires_grad_(True)
+    dy = torch.randn(*lead, fout, generator=g, device="cuda").to(dtype)
+    y = fp8.linear_fp8(x, w)
+    assert y.dtype is dtype and y.shape == (*lead, fout)
+    y.backward(dy)
+    x2, dy2 = x.detach().reshape(-1, fin), dy.reshape(-1, fout)
+    check_product(y.detach().reshape(-1, fout), trip(x2, "row"), trip(w, "tile").t())
+    check_product(x.grad.reshape(-1, fin), trip(dy2, "row"), trip(w, "tile"))
+    check_product(w.grad, trip(dy2, "col").t(), trip(x2, "tile"))
+    # with the weight's encoding at hand, and only one of the gradients
+    q = fp8.quantize_fp8(w.detach(), "tile")
+    (dx,) = torch.autograd.grad(fp8.linear_fp8(x, w.detach(), w_fp8=q), (x,), dy)
+    (dw,) = torch.autograd.grad(fp8.linear_fp8(x.detach(), w, w_fp8=q), (w,), dy)
+    assert torch.equal(dx, x.grad) and torch.equal(dw, w.grad)
+
+
+def test_linear_layer_follows_differences():
+    """The gradients against those of the layer in 64 bits without any 8-bit trip: two operands off by 2 ** -4 of each
+    value at most (2 ** -10 of the block's largest below that) leave the products' errors independent, so the norms agree to
+    2 ** -4 * sqrt(2) at the very most; central differences of a bilinear map are the map itself."""
+    g = torch.Generator(device="cuda").manual_seed(0)
+    x = torch.randn(256, 384, generator=g, device="cuda", dtype=torch.bfloat16).requires_grad_(True)
+    w = (torch.randn(200, 384, generator=g, device="cuda") * 0.05).requires_grad_(True)
+    dy = torch.randn(256, 200, generator=g, device="cuda", dtype=torch.bfloat16)
+    fp8.linear_fp8(x, w).backward(dy)
+    f = lambda a, b: ((a @ b.t()) * dy.double()).sum()                                               # noqa: E731
+    x0, w0 = x.detach().double(), w.detach().double()
+    for grad, direction in ((x.grad, 0), (w.grad, 1)):
+        v = torch.randn(x0.shape if direction == 0 else w0.shape, generator=g, device="cuda").double()
+        v = v + grad.double() / grad.double().norm() * v.norm()             # a direction along which the slope is not small
+        h = 0.5
+        up, down = (f(x0 + h * v, w0), f(x0 - h * v, w0)) if direction == 0 else (f(x0, w0 + h * v), f(x0, w0 - h * v))
+        slope = float((up - down) / (2 * h))
+        assert abs(float((grad.double() * v).sum()) - slope) <= 2.0 ** -4 * 2 ** 0.5 * abs(slope)
+
+
+def test_linear_layer_without_tokens_and_without_gradients():
+    w = torch.randn(64, 96, device="cuda", requires_grad=True)
+    x = torch.randn(0, 96, device="cuda", requires_grad=True)
+    y = fp8.linear_fp8(x, w)
+    y.sum().backward()
+    assert y.shape == (0, 64) and x.grad.shape == (0, 96) and bool((w.grad == 0).all())
+    with torch.no_grad():
+        assert not fp8.linear_fp8(torch.randn(5, 96, device="cuda"), w).requires_grad
+
+
+def test_saved_tensor_hooks_may_change_the_layout():
+    x = torch.randn(130, 300, device="cuda", requires_grad=True)
+    w = torch.randn(70, 300, device="cuda", requires_grad=True)
+    dy = torch.randn(130, 70, device="cuda")
+    want = torch.autograd.grad(c8.silu8(fp8.linear_fp8(x, w)), (x, w), dy)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t.t().contiguous().cuda().t()):
+        y = c8.silu8(fp8.linear_fp8(x, w))
+    for a, b in zip(torch.autograd.grad(y, (x, w), dy), want):
+        assert torch.equal(a, b)
+
+
+def test_training_step_in_a_graph():
+    """Forward and backward captured once and replayed on other data give what the eager step gives."""
+    g = torch.Generator(device="cuda").manual_seed(5)
+    w1 = (torch.randn(256, 384, generator=g, device="cuda") * 0.05).bfloat16().requires_grad_(True)
+    w2 = (torch.randn(384, 256, generator=g, device="cuda") * 0.05).bfloat16().requires_grad_(True)
+    x = torch.randn(100, 384, generator=g, device="cuda").bfloat16()
+    dy = torch.randn(100, 384, generator=g, device="cuda").bfloat16()
+    step = lambda: torch.autograd.grad(fp8.linear_fp8(c8.silu8(fp8.linear_fp8(x, w1)), w2), (w1, w2), dy)   # noqa: E731
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    x.copy_(torch.randn(100, 384, generator=g, device="cuda") * 2)
+    dy.copy_(torch.randn(100, 384, generator=g, device="cuda"))
+    graph.replay()
+    torch.cuda.synchronize()
+    kept = [t.clone() for t in got]
+    for a, b in zip(kept, step()):
+        assert torch.equal(a, b)
+
+
+# ---- activations kept in 8 bits --------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("shape", [(1, 1), (1, 5000), (5, 129), (33, 1001), (2, 17, 256), (300, 1792)])
+def test_activation_against_64_bits(shape, gated, dtype):
+    g = torch.Generator(device="cuda").manual_seed(shape[-1])
+    both = (torch.randn(*shape[:-1], 2 * shape[-1], generator=g, device="cuda") * 4).to(dtype)
+    h, u = (both[..., :shape[-1]], both[..., shape[-1]:]) if gated else (both[..., :shape[-1]].contiguous(), None)
+    dy = torch.randn(shape, generator=g, device="cuda").to(dtype)
+    if gated:
+        y, saved = c8.swiglu8_forward(h, u)
+        dh, du, again = c8.swiglu8_backward(saved, dy, act=True)
+        kept = saved
+    else:
+        y, saved = c8.silu8_forward(h)
+        dh, again = c8.silu8_backward(saved, dy, act=True)
+        kept = (saved,)
+    for k, t in zip(kept, (h, u)):
+        same_encoding((k.data, k.scale), t.reshape(-1, shape[-1]), "row")
+    info = torch.finfo(dtype)
+    # fp32 tensors: about ten roundings of 2 ** -24; 16-bit ones: exponential and quotient within 1e-5
+    rel = 2.0 ** -20 if dtype is torch.float32 else 1e-5
+
+    def close(got, want, mag):
+        tol = mag * rel * (1 + info.eps) + want.abs() * info.eps / 2 + info.smallest_normal * info.eps + 1e-37
+        assert bool(((got.double() - want).abs() <= tol).all())
+
+    hd, ud = h.double(), u.double() if gated else 1.0
+    close(y, hd * torch.sigmoid(hd) * ud, (hd * torch.sigmoid(hd) * ud).abs())
+    hk = kept[0].restore(torch.float32).double()
+    uk = kept[1].restore(torch.float32).double() if gated else torch.ones_like(hk)
+    p = torch.sigmoid(hk)
+    d = dy.double() * uk
+    close(dh, d * (p + hk * p * (1 - p)), d.abs() * (p + hk.abs() * p))
+    close(again, hk * p * uk, (hk * p * uk).abs())
+    if gated:
+        close(du, dy.double() * hk * p, (dy.double() * hk * p).abs())
+    # the autograd forms are the same kernels
+    ins = [t.detach().clone().requires_grad_(True) for t in ((h, u) if gated else (h,))]
+    z = c8.swiglu8(*ins) if gated else c8.silu8(*ins)
+    z.backward(dy)
+    assert torch.equal(z.detach(), y) and torch.equal(ins[0].grad, dh)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_activation_of_extreme_values(dtype):
+    top = torch.finfo(dtype).max
+    h = torch.tensor([[-top, -200.0, -88.0, -0.0, 0.0, 88.0, 200.0, top] * 40], dtype=dtype, device="cuda")
+    y, saved = c8.silu8_forward(h)
+    assert bool(y.isfinite().all()) and float(y[0, -1]) == top
+    d = c8.silu8_backward(saved, torch.ones_like(h))
+    assert bool(d.isfinite().all())
+    h[0, 200] = float("nan")
+    h[0, 3] = float("inf")
+    y, saved = c8.silu8_forward(h)
+    back = saved.restore()
+    assert int(y.isnan().sum()) == 1 and int(back.isnan().sum()) == 2 and bool(back[0, 3].isnan())
+    assert int(c8.silu8_backward(saved, torch.ones_like(h)).isnan().sum()) == 2
+
+
+def test_activation_on_another_stream():
+    s = torch.cuda.Stream()
+    h = torch.randn(500, 700, device="cuda", dtype=torch.bfloat16)
+    want = c8.silu8_forward(h)[0]
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = [c8.silu8_forward(h)[0] for _ in range(5)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(t, want) for t in got)
