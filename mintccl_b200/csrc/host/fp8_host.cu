@@ -161,15 +161,15 @@ int mt_gemm_fp8(void* stream, const void* A, int64_t lda, const void* sa, int64_
     int dev = 0;
     cudaGetDevice(&dev);
     const int sms = nctas > 0 ? nctas : mthost::sm_count(dev);
-    const int64_t mt_ = (M + 127) / 128;
-    const int bn = mt_ * ((N + 255) / 256) >= sms ? 256 : 128;
-    const int64_t tiles = mt_ * ((N + bn - 1) / bn);
+    const bool pair = M > 128 && sms > 1 && (M + 255) / 256 * ((N + 255) / 256) * 4 >= sms;
+    const int bn = pair ? 256 : 128, bm = pair ? 256 : 128;
+    const int64_t tiles = (M + bm - 1) / bm * ((N + bn - 1) / bn);
     if (tiles > 0x3fffffffll) return fail("GEMM shape: too many tiles");
     mt::Fp8GemmArgs a;
     memset(&a, 0, sizeof(a));
     // K-major: boxes of 128 K x the tile's rows; stored transposed: 128 columns x 128 K rows
     if (ta ? mthost::make_u8_map(&a.a, A, K, M, lda, 128) : mthost::make_u8_map(&a.a, A, M, K, lda, 128)) return -1;
-    if (tb ? mthost::make_u8_map(&a.b, B, K, N, ldb, 128) : mthost::make_u8_map(&a.b, B, N, K, ldb, bn)) return -1;
+    if (tb ? mthost::make_u8_map(&a.b, B, K, N, ldb, 128) : mthost::make_u8_map(&a.b, B, N, K, ldb, pair ? bn / 2 : bn)) return -1;
     a.sa = (const float*)sa;
     a.sb = (const float*)sb;
     a.sa_m = sa_m;
@@ -184,7 +184,8 @@ int mt_gemm_fp8(void* stream, const void* A, int64_t lda, const void* sa, int64_
     a.out_dtype = dtype;
     a.vec_out = vec_of(C, ldc, elem_size(dtype)) > 0;
     a.timeout_ns = 4000000000ull;
-    if (launched(mt::launch_fp8_gemm(bn, ta != 0, tb != 0, a, (int)(tiles < sms ? tiles : sms), (cudaStream_t)stream), "fp8 gemm"))
+    const int units = pair ? sms / 2 : sms, used = (int)(tiles < units ? tiles : units);
+    if (launched(mt::launch_fp8_gemm(bn, pair, ta != 0, tb != 0, a, pair ? 2 * used : used, (cudaStream_t)stream), "fp8 gemm"))
       return -1;
     mthost::stat_add(mthost::ST_GEMM, (uint64_t)(2.0 * M * N * K));
     return 0;

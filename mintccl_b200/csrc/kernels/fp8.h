@@ -58,7 +58,8 @@ struct Fp8GemmArgs {
   int32_t vec_out;                  // rows of C start on 16-byte boundaries
   uint64_t timeout_ns;
 };
-cudaError_t launch_fp8_gemm(int bn, bool ta, bool tb, const Fp8GemmArgs& a, int nctas, cudaStream_t s);
+// bn: columns of a tile; pair: tiles of 256 rows on CTA pairs (nctas even), else of 128
+cudaError_t launch_fp8_gemm(int bn, bool pair, bool ta, bool tb, const Fp8GemmArgs& a, int nctas, cudaStream_t s);
 int fp8_gemm_error();   // 1 after a wait of the kernel expired (synchronises), -1 on a CUDA error
 
 }  // namespace mt

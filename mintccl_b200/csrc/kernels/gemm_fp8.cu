@@ -8,9 +8,13 @@
 // Operands may be stored transposed, as in gemm_tc2.cu: the two gradients of a linear layer contract over a dimension
 // that is not the contiguous one.
 //
-//   warps 0..7  sums: a thread has one row and half of the tile's columns; then they store C
-//   warp 8      TMA producer: 128 rows of A and BN of B a stage, 128 bytes each
-//   warp 9      issues tcgen05.mma: four a stage; commits to "stage empty" and "accumulator full"
+// PAIR: two CTAs of a cluster share one tile of 256 rows (cta_group::2), each with its 128 rows of A, half of the tile's
+// rows of B and its half of the accumulator; the leader (cluster rank 0) issues for both.
+//
+//   warps 0..7   sums: a thread has one row and half of the tile's columns; then they store C
+//   warp 8       TMA producer: own halves of A and B; the bytes of both CTAs count on the leader's "stage full" barrier
+//   warp 9       (leader) issues tcgen05.mma: four a stage; commits to "stage empty" and "accumulator full" of both CTAs
+//   warps 10, 11 scales: the products sa * sb of a block for the CTA's rows and both halves, blocks ahead of their use
 //
 // Every wait is bounded; on expiry the CTA raises its abort flag, all roles leave their loops, TMEM is freed and a
 // device-side error word is set for the host.
@@ -30,23 +34,32 @@ namespace mt {
 using namespace tc;
 namespace fp8g {
 
-constexpr int BM = 128, BK = 128;
-constexpr int kSumWarps = 8, kThreads = 32 * (kSumWarps + 2);
-constexpr uint32_t A_BYTES = BM * BK, CHUNK = 128 * 128, TMEM_COLS = 512;
+constexpr int BM = 128, BK = 128;   // rows of a CTA
+constexpr int kSumWarps = 8, kSumThreads = 32 * kSumWarps, kThreads = kSumThreads + 128;
+// Registers a thread after the split of the launch's own; the launch has to bring at least kRegsLaunch (checked on the host).
+constexpr int kRegsSum = 224, kRegsRest = 56, kRegsLaunch = 168;
+static_assert(kRegsSum * kSumThreads + kRegsRest * 128 <= kRegsLaunch * kThreads, "registers of the CTA");
+constexpr int kScaleSlots = 16, kScaleStep = 4;   // blocks whose scales wait in shared memory, and are fetched at a time
+constexpr int kPitch = 144;         // bytes of a staged row of C: 128 and padding
+constexpr uint32_t A_BYTES = BM * BK, TMEM_COLS = 512;
 
-template <int BN>
+template <int BN, bool PAIR>
 struct Shape {
-  static constexpr int STAGES = BN == 256 ? 4 : 6;
-  static constexpr int ACC = BN == 256 ? 2 : 4;   // accumulators in TMEM
-  static constexpr uint32_t B_BYTES = BN * BK;
-  static constexpr uint32_t SMEM = 1024 + STAGES * (A_BYTES + B_BYTES) + 256;
+  static constexpr int BNC = PAIR ? BN / 2 : BN;          // rows of B staged by a CTA
+  static constexpr uint32_t B_BYTES = BNC * BK;
+  static constexpr int STAGES = A_BYTES + B_BYTES > 40000 ? 3 : 5;
+  static constexpr int ACC = BN > 128 ? 2 : 4;            // accumulators in TMEM
+  static constexpr uint32_t OPERANDS = STAGES * (A_BYTES + B_BYTES);
+  static constexpr uint32_t RING = kScaleSlots * 2 * BM * 4, STAGING = kSumWarps * 32 * kPitch;
+  static constexpr uint32_t SMEM = 1024 + OPERANDS + RING + STAGING + 512;
+  static_assert(SMEM <= 232448, "shared memory of one CTA");
 };
 struct Ctl {
-  uint64_t full[6], empty[6], acc_full[4], acc_empty[4], drain;
+  uint64_t full[5], empty[5], acc_full[4], acc_empty[4], sf_full[kScaleSlots], sf_empty[kScaleSlots], drain;
   uint32_t tmem_base;
   int abort;
 };
-static_assert(sizeof(Ctl) <= 256, "control block");
+static_assert(sizeof(Ctl) <= 512, "control block");
 
 __device__ int g_error;
 
@@ -64,7 +77,6 @@ __device__ __forceinline__ float2 unpack2(uint64_t v) {
 __device__ __forceinline__ void fma2(uint64_t& acc, uint64_t p, uint64_t f) {
   asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(p), "l"(f));
 }
-
 // Tile t: groups of 16 row blocks, in a group row block fastest, so that a wave's operands stay in the L2.
 __device__ __forceinline__ void tile_of(int t, int mt_, int nt, int* mb, int* nb) {
   const int per = 16 * nt, gr = t / per, in = t - gr * per, rows = min(16, mt_ - gr * 16);
@@ -72,43 +84,83 @@ __device__ __forceinline__ void tile_of(int t, int mt_, int nt, int* mb, int* nb
   *mb = gr * 16 + in - *nb * rows;
 }
 
-// 32 sums of one row to C: whole vectors, or elements where the row is not aligned or ends.
-template <class T>
-__device__ __forceinline__ void store32(uint8_t* p, const uint64_t* acc, int n, bool vec) {
+// The sums of a warp's 32 rows and CW columns to C.  Whole aligned rows go through shared memory, 128 bytes of every row at
+// a time, so that stores are whole lines; otherwise by elements.
+template <class T, int CW>
+__device__ __forceinline__ void store_sums(const Fp8GemmArgs& a, const uint64_t* acc, uint8_t* stg, int row0, int col, int lane) {
   using E = typename T::elem;
-  float f[32];
+  constexpr int kE = (int)sizeof(E), kPer = 128 / kE, kRounds = (CW + kPer - 1) / kPer;   // columns of a round
+  const int n = a.N - col, rows = a.M - row0;   // may exceed the warp's part
+  uint8_t* base = (uint8_t*)a.c + ((int64_t)row0 * a.ldc + col) * kE;
+  if (a.vec_out && n >= CW) {
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const float2 t = unpack2(acc[i]);
-    f[2 * i] = t.x;
-    f[2 * i + 1] = t.y;
-  }
-  if (vec && n >= 32) {
-    constexpr int kPer = 2 * T::kPer64;   // elements of a 16-byte vector
+    for (int r = 0; r < kRounds; ++r) {
+      constexpr int kTail = CW % kPer;
+      const int cols = r == kRounds - 1 && kTail ? kTail : kPer;
+      uint4* mine = (uint4*)(stg + lane * kPitch);
 #pragma unroll
-    for (int i = 0; i < 32 / kPer; ++i) {
-      const uint64_t lo = T::pack(f + i * kPer), hi = T::pack(f + i * kPer + T::kPer64);
-      *(uint4*)(p + 16 * i) = make_uint4((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
+      for (int j = 0; j < 8; ++j) {
+        if (j * 16 < cols * kE) {
+          uint32_t w[4];
+          const uint64_t* s = acc + (r * kPer + j * 16 / kE) / 2;
+          if constexpr (kE == 4) {
+            const float2 x = unpack2(s[0]), y = unpack2(s[1]);
+            w[0] = __float_as_uint(x.x);
+            w[1] = __float_as_uint(x.y);
+            w[2] = __float_as_uint(y.x);
+            w[3] = __float_as_uint(y.y);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const float2 x = unpack2(s[2 * i]), y = unpack2(s[2 * i + 1]);
+              const float f[4] = {x.x, x.y, y.x, y.y};
+              const uint64_t v = T::pack(f);
+              w[2 * i] = (uint32_t)v;
+              w[2 * i + 1] = (uint32_t)(v >> 32);
+            }
+          }
+          mine[j] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
+      __syncwarp();
+      const int c16 = lane & 7;
+      if (c16 * 16 < cols * kE) {
+#pragma unroll
+        for (int p = 0; p < 8; ++p) {
+          const int rr = p * 4 + (lane >> 3);
+          if (rr < rows) *(uint4*)(base + ((int64_t)rr * a.ldc + r * kPer) * kE + c16 * 16) = *(const uint4*)(stg + rr * kPitch + c16 * 16);
+        }
+      }
+      __syncwarp();
     }
-  } else {
-    E* e = (E*)p;
+  } else if (lane < rows) {
+    E* e = (E*)base + (int64_t)lane * a.ldc;
 #pragma unroll
-    for (int i = 0; i < 32; ++i)
-      if (i < n) e[i] = float_to_elem<T>(f[i]);
+    for (int i = 0; i < CW / 2; ++i) {
+      const float2 x = unpack2(acc[i]);
+      if (2 * i < n) e[2 * i] = float_to_elem<T>(x.x);
+      if (2 * i + 1 < n) e[2 * i + 1] = float_to_elem<T>(x.y);
+    }
   }
 }
 
-template <int BN, bool TA, bool TB>
+template <int BN, bool PAIR, bool TA, bool TB>
 __global__ void __launch_bounds__(kThreads, 1) gemm_fp8_kernel(const __grid_constant__ Fp8GemmArgs a) {
-  using S = Shape<BN>;
-  constexpr int STAGES = S::STAGES, ACC = S::ACC, CW = BN / 2;   // CW: columns of a sum thread
+  using S = Shape<BN, PAIR>;
+  constexpr int STAGES = S::STAGES, ACC = S::ACC, BNC = S::BNC, CW = BN / 2;   // CW: columns of a sum thread
   constexpr uint32_t B_BYTES = S::B_BYTES;
+  constexpr int kRows = PAIR ? 2 * BM : BM;   // of a tile
+  static_assert(!TB || BNC % 128 == 0, "an operand stored transposed comes in chunks of 128 columns");
   extern __shared__ uint8_t smem_raw[];
+  // the same offsets in both CTAs: the MMA descriptors name shared memory of the pair by offset
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* sA = smem;
   uint8_t* sB = smem + STAGES * A_BYTES;
-  Ctl* ctl = (Ctl*)(smem + STAGES * (A_BYTES + B_BYTES));
+  float* sScale = (float*)(smem + S::OPERANDS);
+  uint8_t* sOut = (uint8_t*)sScale + S::RING;
+  Ctl* ctl = (Ctl*)(sOut + S::STAGING);
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+  const int cr = PAIR ? (int)cluster_ctarank() : 0;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -117,7 +169,11 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_fp8_kernel(const __grid_cons
     }
     for (int s = 0; s < ACC; ++s) {
       mbar_init(&ctl->acc_full[s], 1);
-      mbar_init(&ctl->acc_empty[s], kSumWarps);
+      mbar_init(&ctl->acc_empty[s], PAIR ? 2 * kSumWarps : kSumWarps);   // the leader's counts both CTAs
+    }
+    for (int s = 0; s < kScaleSlots; ++s) {
+      mbar_init(&ctl->sf_full[s], 2);
+      mbar_init(&ctl->sf_empty[s], kSumWarps);
     }
     mbar_init(&ctl->drain, 1);
     ctl->abort = 0;
@@ -125,117 +181,190 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_fp8_kernel(const __grid_cons
     tma_prefetch_desc(&a.a);
     tma_prefetch_desc(&a.b);
   }
-  if (warp == 9) {
-    tmem_alloc(&ctl->tmem_base, TMEM_COLS);
-    tmem_relinquish();
+  if (warp == kSumWarps + 1) {
+    if (PAIR) {
+      tmem_alloc_pair(&ctl->tmem_base, TMEM_COLS);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(&ctl->tmem_base, TMEM_COLS);
+      tmem_relinquish();
+    }
   }
   tc_fence_before();
   __syncthreads();
+  if (PAIR) cluster_sync_all();   // both CTAs' barriers exist before anybody signals across
   tc_fence_after();
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, ctl->tmem_base, 0);
   volatile int* abort_flag = &ctl->abort;
-  const int mt_ = (a.M + BM - 1) / BM, nt = (a.N + BN - 1) / BN, tiles = mt_ * nt, kblocks = (a.K + BK - 1) / BK;
+  const int mt_ = (a.M + kRows - 1) / kRows, nt = (a.N + BN - 1) / BN, tiles = mt_ * nt, kblocks = (a.K + BK - 1) / BK;
+  const int first = PAIR ? blockIdx.x >> 1 : blockIdx.x, step = PAIR ? gridDim.x >> 1 : gridDim.x;
 
-  if (warp == 8) {
-    // ------------------------------------------------------------ TMA producer: a uniform warp, one lane issues
-    uint32_t s = 0, ph = 0;
-    bool ok = true;
-    for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
-      int mb, nb;
-      tile_of(t, mt_, nt, &mb, &nb);
-      for (int kb = 0; kb < kblocks; ++kb) {
-        if (!wait_bar_warp(&ctl->empty[s], ph ^ 1, abort_flag, a.timeout_ns)) {
-          ok = false;
-          break;
-        }
-        if (elect_one()) {
-          mbar_expect_tx(&ctl->full[s], A_BYTES + B_BYTES);
-          if (TA) tma_load_2d(sA + s * A_BYTES, &a.a, mb * BM, kb * BK, &ctl->full[s]);
-          else tma_load_2d(sA + s * A_BYTES, &a.a, kb * BK, mb * BM, &ctl->full[s]);
-          if (TB) {
+  if (warp >= kSumWarps) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsRest));
+    if (warp == kSumWarps) {
+      // ---------------------------------------------------------- TMA producer: a uniform warp, one lane issues
+      const uint32_t full_leader = map_to_cta(smem_u32(&ctl->full[0]), 0);
+      uint32_t s = 0, ph = 0;
+      bool ok = true;
+      auto load = [&](uint8_t* dst, const CUtensorMap* map, int x, int y) {
+        if (PAIR) tma_load_2d_pair(dst, map, x, y, full_leader + s * 8);
+        else tma_load_2d(dst, map, x, y, &ctl->full[s]);
+      };
+      for (int t = first; ok && t < tiles; t += step) {
+        int mb, nb;
+        tile_of(t, mt_, nt, &mb, &nb);
+        const int arow = mb * kRows + cr * BM, brow = nb * BN + cr * BNC;
+        for (int kb = 0; kb < kblocks; ++kb) {
+          if (!wait_bar_warp(&ctl->empty[s], ph ^ 1, abort_flag, a.timeout_ns)) {
+            ok = false;
+            break;
+          }
+          if (elect_one()) {
+            if (cr == 0) mbar_expect_tx(&ctl->full[s], (PAIR ? 2 : 1) * (A_BYTES + B_BYTES));
+            if (TA) load(sA + s * A_BYTES, &a.a, arow, kb * BK);
+            else load(sA + s * A_BYTES, &a.a, kb * BK, arow);
+            if (TB) {
 #pragma unroll
-            for (int c = 0; c < BN / 128; ++c)
-              tma_load_2d(sB + s * B_BYTES + c * CHUNK, &a.b, nb * BN + c * 128, kb * BK, &ctl->full[s]);
-          } else {
-            tma_load_2d(sB + s * B_BYTES, &a.b, kb * BK, nb * BN, &ctl->full[s]);
+              for (int c = 0; c < BNC / 128; ++c) load(sB + s * B_BYTES + c * (128 * BK), &a.b, brow + c * 128, kb * BK);
+            } else {
+              load(sB + s * B_BYTES, &a.b, kb * BK, brow);
+            }
+          }
+          __syncwarp();
+          if (++s == STAGES) {
+            s = 0;
+            ph ^= 1;
           }
         }
-        __syncwarp();
-        if (++s == STAGES) {
-          s = 0;
-          ph ^= 1;
-        }
       }
-    }
-    if (aborted_warp(abort_flag)) {
-      // copies in flight may still be landing in shared memory: give them a bounded time
-      const uint64_t t0 = globaltimer();
-      while (globaltimer() - t0 < 100000ull) __nanosleep(1000);
-    }
-  } else if (warp == 9) {
-    // ------------------------------------------------------------ MMA issuer: uniform, one lane issues
-    constexpr uint32_t idesc = make_idesc_e4m3(BM, BN) | (TA ? kIdescTransA : 0u) | (TB ? kIdescTransB : 0u);
-    // a step of 32 along K: 32 bytes of a row, or 32 rows of 128 bytes
-    constexpr uint64_t step_a = TA ? 256 : 2, step_b = TB ? 256 : 2;
-    uint32_t s = 0, ph = 0, b = 0, bph = 0;
-    bool ok = true;
-    for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
-      for (int kb = 0; kb < kblocks; ++kb) {
-        if (!wait_bar_warp(&ctl->acc_empty[b], bph ^ 1, abort_flag, a.timeout_ns) ||
-            !wait_bar_warp(&ctl->full[s], ph, abort_flag, a.timeout_ns)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        const uint64_t da = TA ? make_smem_desc_mn_sw128(sA + s * A_BYTES, CHUNK) : make_smem_desc_sw128(sA + s * A_BYTES);
-        const uint64_t db = TB ? make_smem_desc_mn_sw128(sB + s * B_BYTES, CHUNK) : make_smem_desc_sw128(sB + s * B_BYTES);
-        if (elect_one()) {
+      if (aborted_warp(abort_flag)) {
+        // copies in flight may still be landing in shared memory: give them a bounded time
+        const uint64_t t0 = globaltimer();
+        while (globaltimer() - t0 < 100000ull) __nanosleep(1000);
+      }
+    } else if (warp == kSumWarps + 1 && cr == 0) {
+      // ---------------------------------------------------------- MMA issuer: uniform, one lane issues
+      constexpr uint32_t idesc = make_idesc_e4m3(kRows, BN) | (TA ? kIdescTransA : 0u) | (TB ? kIdescTransB : 0u);
+      // a step of 32 along K: 32 bytes of a row, or 32 rows of 128 bytes
+      constexpr uint64_t step_a = TA ? 256 : 2, step_b = TB ? 256 : 2;
+      uint32_t s = 0, ph = 0, b = 0, bph = 0;
+      bool ok = true;
+      auto commit = [&](uint64_t* bar) {
+        if (PAIR) umma_commit_both(bar);
+        else umma_commit(bar);
+      };
+      for (int t = first; ok && t < tiles; t += step) {
+        for (int kb = 0; kb < kblocks; ++kb) {
+          if (!wait_bar_warp(&ctl->acc_empty[b], bph ^ 1, abort_flag, a.timeout_ns) ||
+              !wait_bar_warp(&ctl->full[s], ph, abort_flag, a.timeout_ns)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint64_t da = TA ? make_smem_desc_mn_sw128(sA + s * A_BYTES, 128 * BK) : make_smem_desc_sw128(sA + s * A_BYTES);
+          const uint64_t db = TB ? make_smem_desc_mn_sw128(sB + s * B_BYTES, 128 * BK) : make_smem_desc_sw128(sB + s * B_BYTES);
+          if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            umma_f8(tmem_base + b * BN, da + k * step_a, db + k * step_b, idesc, k > 0 ? 1u : 0u);
-          umma_commit(&ctl->empty[s]);
-          umma_commit(&ctl->acc_full[b]);
+            for (int k = 0; k < 4; ++k) {
+              if (PAIR) umma_f8_pair(tmem_base + b * BN, da + k * step_a, db + k * step_b, idesc, k > 0 ? 1u : 0u);
+              else umma_f8(tmem_base + b * BN, da + k * step_a, db + k * step_b, idesc, k > 0 ? 1u : 0u);
+            }
+            commit(&ctl->empty[s]);
+            commit(&ctl->acc_full[b]);
+          }
+          __syncwarp();
+          if (++s == STAGES) {
+            s = 0;
+            ph ^= 1;
+          }
+          if (++b == ACC) {
+            b = 0;
+            bph ^= 1;
+          }
         }
-        __syncwarp();
-        if (++s == STAGES) {
-          s = 0;
-          ph ^= 1;
-        }
-        if (++b == ACC) {
-          b = 0;
-          bph ^= 1;
+      }
+      // no MMA may still be writing TMEM when it is freed
+      if (elect_one()) {
+        if (PAIR) umma_commit_pair(smem_u32(&ctl->drain));
+        else umma_commit(&ctl->drain);
+      }
+      __syncwarp();
+      wait_bar_warp(&ctl->drain, 0, abort_flag, a.timeout_ns);
+    } else if (warp >= kSumWarps + 2) {
+      // ---------------------------------------------------------- scales: a lane has two rows, 64 apart
+      const int r = (warp - kSumWarps - 2) * 32 + lane;
+      uint32_t s = 0, ph = 0;
+      bool ok = true;
+      for (int t = first; ok && t < tiles; t += step) {
+        int mb, nb;
+        tile_of(t, mt_, nt, &mb, &nb);
+        const int row = mb * kRows + cr * BM + r, c0 = nb * BN, c1 = c0 + CW;
+        const float* pa0 = a.sa + (int64_t)(row < a.M ? row : 0) * a.sa_m;
+        const float* pa1 = a.sa + (int64_t)(row + 64 < a.M ? row + 64 : 0) * a.sa_m;
+        const float* pb0 = a.sb + (int64_t)(c0 >> 7) * a.sb_n;
+        const float* pb1 = a.sb + (int64_t)(c1 < a.N ? c1 >> 7 : 0) * a.sb_n;
+        for (int kb = 0; ok && kb < kblocks; kb += kScaleStep) {
+          float va[kScaleStep][2], vb[kScaleStep][2];
+#pragma unroll
+          for (int i = 0; i < kScaleStep; ++i) {
+            const int64_t k = min(kb + i, kblocks - 1);
+            va[i][0] = __ldg(pa0 + k * a.sa_k);
+            va[i][1] = __ldg(pa1 + k * a.sa_k);
+            vb[i][0] = __ldg(pb0 + k * a.sb_k);
+            vb[i][1] = __ldg(pb1 + k * a.sb_k);
+          }
+#pragma unroll
+          for (int i = 0; i < kScaleStep; ++i) {
+            if (!ok || kb + i >= kblocks) break;
+            ok = wait_bar_warp(&ctl->sf_empty[s], ph ^ 1, abort_flag, a.timeout_ns);
+            float* f = sScale + s * (2 * BM) + r;
+            f[0] = va[i][0] * vb[i][0];
+            f[64] = va[i][1] * vb[i][0];
+            f[BM] = va[i][0] * vb[i][1];
+            f[BM + 64] = va[i][1] * vb[i][1];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&ctl->sf_full[s]);
+            if (++s == kScaleSlots) {
+              s = 0;
+              ph ^= 1;
+            }
+          }
         }
       }
     }
-    // no MMA may still be writing TMEM when it is freed
-    if (elect_one()) umma_commit(&ctl->drain);
-    __syncwarp();
-    wait_bar_warp(&ctl->drain, 0, abort_flag, a.timeout_ns);
   } else {
     // ------------------------------------------------------------ sums and C
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSum));
     const int q = warp & 3, half = warp >> 2;   // TMEM lane quarter, half of the columns
+    const uint32_t empty_leader = map_to_cta(smem_u32(&ctl->acc_empty[0]), 0);
+    uint8_t* stg = sOut + warp * 32 * kPitch;
+    const float* factor = sScale + half * BM + q * 32 + lane;
+    uint32_t sf = 0, sph = 0;
     uint32_t b = 0, bph = 0;
     bool ok = true;
-    for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
+    for (int t = first; ok && t < tiles; t += step) {
       int mb, nb;
       tile_of(t, mt_, nt, &mb, &nb);
-      const int row = mb * BM + q * 32 + lane, col = nb * BN + half * CW;
-      const bool live = row < a.M, work = mb * BM + q * 32 < a.M && col < a.N;   // work: the same for the whole warp
-      const float* pa = a.sa + (int64_t)row * a.sa_m;
-      const float* pb = a.sb + (int64_t)(col >> 7) * a.sb_n;
+      const int row0 = mb * kRows + cr * BM + q * 32, col = nb * BN + half * CW;
+      const bool work = row0 < a.M && col < a.N;   // the same for the whole warp
       uint64_t acc[CW / 2];
 #pragma unroll
       for (int i = 0; i < CW / 2; ++i) acc[i] = 0;
-      float fa = live ? __ldg(pa) : 0.f, fb = work ? __ldg(pb) : 0.f;
       for (int kb = 0; kb < kblocks; ++kb) {
-        const float f = fa * fb;
-        if (kb + 1 < kblocks) {   // the next block's scales arrive while this one is waited for
-          fa = live ? __ldg(pa + (int64_t)(kb + 1) * a.sa_k) : 0.f;
-          fb = work ? __ldg(pb + (int64_t)(kb + 1) * a.sb_k) : 0.f;
-        }
-        if (!wait_bar_warp(&ctl->acc_full[b], bph, abort_flag, a.timeout_ns)) {
+        if (!wait_bar(&ctl->sf_full[sf], sph, abort_flag, a.timeout_ns)) {
           ok = false;
           break;
+        }
+        const float f = factor[sf * (2 * BM)];
+        if (!wait_bar(&ctl->acc_full[b], bph, abort_flag, a.timeout_ns)) {
+          ok = false;
+          break;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ctl->sf_empty[sf]);
+        if (++sf == kScaleSlots) {
+          sf = 0;
+          sph ^= 1;
         }
         if (work) {
           tc_fence_after();
@@ -253,62 +382,77 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_fp8_kernel(const __grid_cons
           tc_fence_before();
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&ctl->acc_empty[b]);
+        if (lane == 0) {
+          if (PAIR) mbar_arrive_cluster(empty_leader + b * 8);
+          else mbar_arrive(&ctl->acc_empty[b]);
+        }
         if (++b == ACC) {
           b = 0;
           bph ^= 1;
         }
       }
-      if (ok && live && work) {
-        const int esz = a.out_dtype == DT_F32 ? 4 : 2;
-        uint8_t* p = (uint8_t*)a.c + ((int64_t)row * a.ldc + col) * esz;
-#pragma unroll
-        for (int c = 0; c < CW / 32; ++c) {
-          const int n = a.N - col - c * 32;
-          if (n > 0) {
-            if (a.out_dtype == DT_F32) store32<F32>(p + c * 128, acc + c * 16, n, a.vec_out);
-            else if (a.out_dtype == DT_BF16) store32<BF16>(p + c * 64, acc + c * 16, n, a.vec_out);
-            else store32<F16>(p + c * 64, acc + c * 16, n, a.vec_out);
-          }
-        }
+      if (ok && work) {
+        if (a.out_dtype == DT_F32) store_sums<F32, CW>(a, acc, stg, row0, col, lane);
+        else if (a.out_dtype == DT_BF16) store_sums<BF16, CW>(a, acc, stg, row0, col, lane);
+        else store_sums<F16, CW>(a, acc, stg, row0, col, lane);
       }
     }
   }
 
+  // ---------------------------------------------------------------- tear-down
   tc_fence_before();
   __syncthreads();
-  if (warp == 9) {
-    tc_fence_after();
-    tmem_dealloc(tmem_base, TMEM_COLS);
+  if (threadIdx.x == 0 && *abort_flag) {
+    if (PAIR) st_cluster_u32(map_to_cta(smem_u32(&ctl->abort), cr ^ 1), 1u);   // the peer would notice after its own time limit
+    atomicExch(&g_error, 1);
   }
-  if (threadIdx.x == 0 && *abort_flag) atomicExch(&g_error, 1);
+  if (PAIR) cluster_sync_all();   // neither CTA leaves, or frees TMEM, while the other may still signal into it
+  if (warp == kSumWarps + 1) {
+    tc_fence_after();
+    if (PAIR) tmem_dealloc_pair(tmem_base, TMEM_COLS);
+    else tmem_dealloc(tmem_base, TMEM_COLS);
+  }
 }
 
-template <int BN, bool TA, bool TB>
+template <int BN, bool PAIR, bool TA, bool TB>
 cudaError_t go(const Fp8GemmArgs& a, int nctas, cudaStream_t s) {
-  const void* fn = (const void*)gemm_fp8_kernel<BN, TA, TB>;
+  const void* fn = (const void*)gemm_fp8_kernel<BN, PAIR, TA, TB>;
+  // the register split waits forever for registers that the launch did not bring
+  static const int regs = [&] {
+    cudaFuncAttributes at;
+    return cudaFuncGetAttributes(&at, fn) == cudaSuccess ? at.numRegs : 0;
+  }();
+  if (regs < kRegsLaunch) return cudaErrorLaunchOutOfResources;
   // per device, and cheap enough to say at every launch
-  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<BN>::SMEM);
+  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<BN, PAIR>::SMEM);
   if (e != cudaSuccess) return e;
-  gemm_fp8_kernel<BN, TA, TB><<<nctas, kThreads, Shape<BN>::SMEM, s>>>(a);
-  return cudaGetLastError();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(nctas);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = Shape<BN, PAIR>::SMEM;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = PAIR ? 2 : 1;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, gemm_fp8_kernel<BN, PAIR, TA, TB>, a);
 }
-template <int BN>
+template <int BN, bool PAIR>
 cudaError_t go_form(bool ta, bool tb, const Fp8GemmArgs& a, int nctas, cudaStream_t s) {
-  if (ta) return go<BN, true, true>(a, nctas, s);
-  return tb ? go<BN, false, true>(a, nctas, s) : go<BN, false, false>(a, nctas, s);
+  if (ta) return go<BN, PAIR, true, true>(a, nctas, s);
+  return tb ? go<BN, PAIR, false, true>(a, nctas, s) : go<BN, PAIR, false, false>(a, nctas, s);
 }
 
 }  // namespace fp8g
 
-cudaError_t launch_fp8_gemm(int bn, bool ta, bool tb, const Fp8GemmArgs& a, int nctas, cudaStream_t s) {
+cudaError_t launch_fp8_gemm(int bn, bool pair, bool ta, bool tb, const Fp8GemmArgs& a, int nctas, cudaStream_t s) {
   if (ta && !tb) return cudaErrorInvalidValue;
   count_launch();
-  switch (bn) {
-    case 256: return fp8g::go_form<256>(ta, tb, a, nctas, s);
-    case 128: return fp8g::go_form<128>(ta, tb, a, nctas, s);
-    default: return cudaErrorInvalidValue;
-  }
+  if (pair && bn == 256) return fp8g::go_form<256, true>(ta, tb, a, nctas, s);
+  if (!pair && bn == 128) return fp8g::go_form<128, false>(ta, tb, a, nctas, s);
+  return cudaErrorInvalidValue;
 }
 
 int fp8_gemm_error() {
