@@ -35,6 +35,18 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
+// The same without ever waiting: a probe whose answer may be used later.
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
 // One lane of a converged warp, the same one every time.  Code around it stays warp-uniform, so that what it computes
 // (descriptors, barrier addresses) lives in uniform registers, where tcgen05 and TMA instructions take their operands.
 __device__ __forceinline__ bool elect_one() {

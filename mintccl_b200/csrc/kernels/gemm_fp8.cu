@@ -39,7 +39,7 @@ constexpr int kSumWarps = 8, kSumThreads = 32 * kSumWarps, kThreads = kSumThread
 // Registers a thread after the split of the launch's own; the launch has to bring at least kRegsLaunch (checked on the host).
 constexpr int kRegsSum = 224, kRegsRest = 56, kRegsLaunch = 168;
 static_assert(kRegsSum * kSumThreads + kRegsRest * 128 <= kRegsLaunch * kThreads, "registers of the CTA");
-constexpr int kScaleSlots = 16, kScaleStep = 4;   // blocks whose scales wait in shared memory, and are fetched at a time
+constexpr int kScaleSlots = 16;     // blocks whose scales wait in shared memory
 constexpr int kPitch = 144;         // bytes of a staged row of C: 128 and padding
 constexpr uint32_t A_BYTES = BM * BK, TMEM_COLS = 512;
 
@@ -51,21 +51,22 @@ struct Shape {
   static constexpr int ACC = BN > 128 ? 2 : 4;            // accumulators in TMEM
   static constexpr uint32_t OPERANDS = STAGES * (A_BYTES + B_BYTES);
   static constexpr uint32_t RING = kScaleSlots * 2 * BM * 4, STAGING = kSumWarps * 32 * kPitch;
-  static constexpr uint32_t SMEM = 1024 + OPERANDS + RING + STAGING + 512;
+  static constexpr uint32_t SMEM = 1024 + OPERANDS + RING + STAGING + 256;
   static_assert(SMEM <= 232448, "shared memory of one CTA");
 };
 struct Ctl {
-  uint64_t full[5], empty[5], acc_full[4], acc_empty[4], sf_full[kScaleSlots], sf_empty[kScaleSlots], drain;
+  uint64_t full[5], empty[5], acc_full[4], acc_empty[4], drain;
   uint32_t tmem_base;
   int abort;
 };
-static_assert(sizeof(Ctl) <= 512, "control block");
+static_assert(sizeof(Ctl) <= 256, "control block");
 
 __device__ int g_error;
 
-__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
+// Two sums in a register pair: one instruction adds to both, which leaves issue slots to the warps that feed the tensor core.
+__device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) {
   uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
   return r;
 }
 __device__ __forceinline__ float2 unpack2(uint64_t v) {
@@ -73,10 +74,10 @@ __device__ __forceinline__ float2 unpack2(uint64_t v) {
   asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
   return r;
 }
-// acc += p * f on two floats at once
 __device__ __forceinline__ void fma2(uint64_t& acc, uint64_t p, uint64_t f) {
   asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(p), "l"(f));
 }
+
 // Tile t: groups of 16 row blocks, in a group row block fastest, so that a wave's operands stay in the L2.
 __device__ __forceinline__ void tile_of(int t, int mt_, int nt, int* mb, int* nb) {
   const int per = 16 * nt, gr = t / per, in = t - gr * per, rows = min(16, mt_ - gr * 16);
@@ -102,22 +103,18 @@ __device__ __forceinline__ void store_sums(const Fp8GemmArgs& a, const uint64_t*
       for (int j = 0; j < 8; ++j) {
         if (j * 16 < cols * kE) {
           uint32_t w[4];
-          const uint64_t* s = acc + (r * kPer + j * 16 / kE) / 2;
-          if constexpr (kE == 4) {
-            const float2 x = unpack2(s[0]), y = unpack2(s[1]);
-            w[0] = __float_as_uint(x.x);
-            w[1] = __float_as_uint(x.y);
-            w[2] = __float_as_uint(y.x);
-            w[3] = __float_as_uint(y.y);
-          } else {
+          float f[16 / kE];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const float2 x = unpack2(s[2 * i]), y = unpack2(s[2 * i + 1]);
-              const float f[4] = {x.x, x.y, y.x, y.y};
-              const uint64_t v = T::pack(f);
-              w[2 * i] = (uint32_t)v;
-              w[2 * i + 1] = (uint32_t)(v >> 32);
-            }
+          for (int i = 0; i < 8 / kE; ++i) {
+            const float2 x = unpack2(acc[(r * kPer + j * 16 / kE) / 2 + i]);
+            f[2 * i] = x.x;
+            f[2 * i + 1] = x.y;
+          }
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint64_t v = T::pack(f + i * T::kPer64);
+            w[2 * i] = (uint32_t)v;
+            w[2 * i + 1] = (uint32_t)(v >> 32);
           }
           mine[j] = make_uint4(w[0], w[1], w[2], w[3]);
         }
@@ -164,16 +161,12 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_fp8_kernel(const __grid_cons
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&ctl->full[s], 1);
+      mbar_init(&ctl->full[s], PAIR ? 3 : 2);   // the producer's byte count and the scales of each CTA
       mbar_init(&ctl->empty[s], 1);
     }
     for (int s = 0; s < ACC; ++s) {
       mbar_init(&ctl->acc_full[s], 1);
       mbar_init(&ctl->acc_empty[s], PAIR ? 2 * kSumWarps : kSumWarps);   // the leader's counts both CTAs
-    }
-    for (int s = 0; s < kScaleSlots; ++s) {
-      mbar_init(&ctl->sf_full[s], 2);
-      mbar_init(&ctl->sf_empty[s], kSumWarps);
     }
     mbar_init(&ctl->drain, 1);
     ctl->abort = 0;
@@ -205,7 +198,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_fp8_kernel(const __grid_cons
       // ---------------------------------------------------------- TMA producer: a uniform warp, one lane issues
       const uint32_t full_leader = map_to_cta(smem_u32(&ctl->full[0]), 0);
       uint32_t s = 0, ph = 0;
-      bool ok = true;
+      bool ok = true, free = true;   // free: a probe found the next stage empty
       auto load = [&](uint8_t* dst, const CUtensorMap* map, int x, int y) {
         if (PAIR) tma_load_2d_pair(dst, map, x, y, full_leader + s * 8);
         else tma_load_2d(dst, map, x, y, &ctl->full[s]);
@@ -215,10 +208,12 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_fp8_kernel(const __grid_cons
         tile_of(t, mt_, nt, &mb, &nb);
         const int arow = mb * kRows + cr * BM, brow = nb * BN + cr * BNC;
         for (int kb = 0; kb < kblocks; ++kb) {
-          if (!wait_bar_warp(&ctl->empty[s], ph ^ 1, abort_flag, a.timeout_ns)) {
+          if (!free && !wait_bar_warp(&ctl->empty[s], ph ^ 1, abort_flag, a.timeout_ns)) {
             ok = false;
             break;
           }
+          const uint32_t sn = s + 1 == STAGES ? 0 : s + 1, phn = s + 1 == STAGES ? ph ^ 1 : ph;
+          free = __all_sync(0xffffffffu, mbar_test(&ctl->empty[sn], phn ^ 1));
           if (elect_one()) {
             if (cr == 0) mbar_expect_tx(&ctl->full[s], (PAIR ? 2 : 1) * (A_BYTES + B_BYTES));
             if (TA) load(sA + s * A_BYTES, &a.a, arow, kb * BK);
@@ -231,10 +226,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_fp8_kernel(const __grid_cons
             }
           }
           __syncwarp();
-          if (++s == STAGES) {
-            s = 0;
-            ph ^= 1;
-          }
+          s = sn;
+          ph = phn;
         }
       }
       if (aborted_warp(abort_flag)) {
@@ -255,8 +248,11 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_fp8_kernel(const __grid_cons
       };
       for (int t = first; ok && t < tiles; t += step) {
         for (int kb = 0; kb < kblocks; ++kb) {
-          if (!wait_bar_warp(&ctl->acc_empty[b], bph ^ 1, abort_flag, a.timeout_ns) ||
-              !wait_bar_warp(&ctl->full[s], ph, abort_flag, a.timeout_ns)) {
+          // both probes in flight at once: each takes some 230 cycles beside the tensor core's own shared-memory traffic
+          const bool drained = mbar_test(&ctl->acc_empty[b], bph ^ 1), loaded = mbar_test(&ctl->full[s], ph);
+          if (!__all_sync(0xffffffffu, drained && loaded) &&
+              (!wait_bar_warp(&ctl->acc_empty[b], bph ^ 1, abort_flag, a.timeout_ns) ||
+               !wait_bar_warp(&ctl->full[s], ph, abort_flag, a.timeout_ns))) {
             ok = false;
             break;
           }
@@ -291,41 +287,51 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_fp8_kernel(const __grid_cons
       __syncwarp();
       wait_bar_warp(&ctl->drain, 0, abort_flag, a.timeout_ns);
     } else if (warp >= kSumWarps + 2) {
-      // ---------------------------------------------------------- scales: a lane has two rows, 64 apart
-      const int r = (warp - kSumWarps - 2) * 32 + lane;
-      uint32_t s = 0, ph = 0;
+      // ---------------------------------------------------------- scales: one warp for even blocks, one for odd; a lane has
+      // four rows, 32 apart.  They count on the stage's "full" barrier: whoever sees the block's accumulator sees them too.
+      // A slot is free when its stage is: the sums are at most ACC + STAGES blocks behind.
+      static_assert(ACC + STAGES < kScaleSlots, "slots of the scales");
+      const int w = warp - kSumWarps - 2;
+      const uint32_t full_leader = map_to_cta(smem_u32(&ctl->full[0]), 0);
+      uint32_t s = w, ph = 0, pos = 0;   // stage of this warp's next block, and the tile's first block among all
       bool ok = true;
-      for (int t = first; ok && t < tiles; t += step) {
+      for (int t = first; ok && t < tiles; t += step, pos += kblocks) {
         int mb, nb;
         tile_of(t, mt_, nt, &mb, &nb);
-        const int row = mb * kRows + cr * BM + r, c0 = nb * BN, c1 = c0 + CW;
-        const float* pa0 = a.sa + (int64_t)(row < a.M ? row : 0) * a.sa_m;
-        const float* pa1 = a.sa + (int64_t)(row + 64 < a.M ? row + 64 : 0) * a.sa_m;
+        const int row = mb * kRows + cr * BM + lane, c0 = nb * BN, c1 = c0 + CW;
+        const float* pa[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) pa[i] = a.sa + (int64_t)(row + 32 * i < a.M ? row + 32 * i : 0) * a.sa_m;
         const float* pb0 = a.sb + (int64_t)(c0 >> 7) * a.sb_n;
         const float* pb1 = a.sb + (int64_t)(c1 < a.N ? c1 >> 7 : 0) * a.sb_n;
-        for (int kb = 0; ok && kb < kblocks; kb += kScaleStep) {
-          float va[kScaleStep][2], vb[kScaleStep][2];
+        for (int kb = (pos + w) & 1; ok && kb < kblocks; kb += 4) {
+          float va[2][4], vb[2][2];
 #pragma unroll
-          for (int i = 0; i < kScaleStep; ++i) {
-            const int64_t k = min(kb + i, kblocks - 1);
-            va[i][0] = __ldg(pa0 + k * a.sa_k);
-            va[i][1] = __ldg(pa1 + k * a.sa_k);
-            vb[i][0] = __ldg(pb0 + k * a.sb_k);
-            vb[i][1] = __ldg(pb1 + k * a.sb_k);
+          for (int j = 0; j < 2; ++j) {
+            const int64_t k = min(kb + 2 * j, kblocks - 1);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) va[j][i] = __ldg(pa[i] + k * a.sa_k);
+            vb[j][0] = __ldg(pb0 + k * a.sb_k);
+            vb[j][1] = __ldg(pb1 + k * a.sb_k);
           }
 #pragma unroll
-          for (int i = 0; i < kScaleStep; ++i) {
-            if (!ok || kb + i >= kblocks) break;
-            ok = wait_bar_warp(&ctl->sf_empty[s], ph ^ 1, abort_flag, a.timeout_ns);
-            float* f = sScale + s * (2 * BM) + r;
-            f[0] = va[i][0] * vb[i][0];
-            f[64] = va[i][1] * vb[i][0];
-            f[BM] = va[i][0] * vb[i][1];
-            f[BM + 64] = va[i][1] * vb[i][1];
+          for (int j = 0; j < 2; ++j) {
+            if (!ok || kb + 2 * j >= kblocks) continue;
+            ok = wait_bar_warp(&ctl->empty[s], ph ^ 1, abort_flag, a.timeout_ns);
+            float* f = sScale + ((pos + kb + 2 * j) & (kScaleSlots - 1)) * (2 * BM) + lane;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              f[32 * i] = va[j][i] * vb[j][0];
+              f[BM + 32 * i] = va[j][i] * vb[j][1];
+            }
             __syncwarp();
-            if (lane == 0) mbar_arrive(&ctl->sf_full[s]);
-            if (++s == kScaleSlots) {
-              s = 0;
+            if (lane == 0) {
+              if (PAIR) mbar_arrive_cluster(full_leader + s * 8);
+              else mbar_arrive(&ctl->full[s]);
+            }
+            s += 2;
+            if (s >= STAGES) {
+              s -= STAGES;
               ph ^= 1;
             }
           }
@@ -339,9 +345,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_fp8_kernel(const __grid_cons
     const uint32_t empty_leader = map_to_cta(smem_u32(&ctl->acc_empty[0]), 0);
     uint8_t* stg = sOut + warp * 32 * kPitch;
     const float* factor = sScale + half * BM + q * 32 + lane;
-    uint32_t sf = 0, sph = 0;
-    uint32_t b = 0, bph = 0;
-    bool ok = true;
+    uint32_t pos = 0, b = 0, bph = 0;
+    bool ok = true, ready = false;   // ready: a probe found the next accumulator full
     for (int t = first; ok && t < tiles; t += step) {
       int mb, nb;
       tile_of(t, mt_, nt, &mb, &nb);
@@ -351,45 +356,39 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_fp8_kernel(const __grid_cons
 #pragma unroll
       for (int i = 0; i < CW / 2; ++i) acc[i] = 0;
       for (int kb = 0; kb < kblocks; ++kb) {
-        if (!wait_bar(&ctl->sf_full[sf], sph, abort_flag, a.timeout_ns)) {
-          ok = false;
-          break;
-        }
-        const float f = factor[sf * (2 * BM)];
-        if (!wait_bar(&ctl->acc_full[b], bph, abort_flag, a.timeout_ns)) {
+        if (!ready && !wait_bar(&ctl->acc_full[b], bph, abort_flag, a.timeout_ns)) {
           ok = false;
           break;
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&ctl->sf_empty[sf]);
-        if (++sf == kScaleSlots) {
-          sf = 0;
-          sph ^= 1;
-        }
-        if (work) {
-          tc_fence_after();
-          const uint64_t f2 = pack2(f, f);
-          const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + b * BN + half * CW;
+        tc_fence_after();
+        // 16 columns at a time: the next ones arrive while these are added, and the accumulator goes back to the tensor
+        // core before the last are
+        const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + b * BN + half * CW;
+        const uint32_t bn = b + 1 == ACC ? 0 : b + 1, bphn = b + 1 == ACC ? bph ^ 1 : bph;
+        uint32_t r[2][16];
+        tmem_ld_32x16(taddr, r[0]);
+        const uint32_t f = __float_as_uint(factor[(pos++ & (kScaleSlots - 1)) * (2 * BM)]);
+        const uint64_t f2 = pack2(f, f);
 #pragma unroll
-          for (int c = 0; c < CW / 32; ++c) {
-            uint32_t r[32];
-            tmem_ld_32x32(taddr + c * 32, r);
-            tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              fma2(acc[c * 16 + i], (uint64_t)r[2 * i] | ((uint64_t)r[2 * i + 1] << 32), f2);
+        for (int c = 0; c < CW / 16; ++c) {
+          tmem_ld_wait();
+          if (c == CW / 16 - 3) ready = mbar_test(&ctl->acc_full[bn], bphn);   // known by the time it is needed
+          if (c + 1 < CW / 16) {
+            tmem_ld_32x16(taddr + (c + 1) * 16, r[(c + 1) & 1]);
+          } else {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+              if (PAIR) mbar_arrive_cluster(empty_leader + b * 8);
+              else mbar_arrive(&ctl->acc_empty[b]);
+            }
           }
-          tc_fence_before();
+#pragma unroll
+          for (int i = 0; i < 8; ++i) fma2(acc[c * 8 + i], pack2(r[c & 1][2 * i], r[c & 1][2 * i + 1]), f2);
         }
-        __syncwarp();
-        if (lane == 0) {
-          if (PAIR) mbar_arrive_cluster(empty_leader + b * 8);
-          else mbar_arrive(&ctl->acc_empty[b]);
-        }
-        if (++b == ACC) {
-          b = 0;
-          bph ^= 1;
-        }
+        b = bn;
+        bph = bphn;
       }
       if (ok && work) {
         if (a.out_dtype == DT_F32) store_sums<F32, CW>(a, acc, stg, row0, col, lane);
