@@ -152,6 +152,12 @@ __device__ __forceinline__ uint64_t make_smem_desc_mn_sw128(const void* smem_til
   const uint64_t addr = (uint64_t)(smem_u32(smem_tile) >> 4) & 0x3fffull;
   return addr | ((uint64_t)(chunk_bytes >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
 }
+// One chunk of 64 bytes (64 columns of 8 bits) with the 64-byte swizzle: groups of 8 K rows are 512 bytes apart, a step of
+// 32 along K is 2048 bytes (128 units).
+__device__ __forceinline__ uint64_t make_smem_desc_mn_sw64(const void* smem_tile) {
+  const uint64_t addr = (uint64_t)(smem_u32(smem_tile) >> 4) & 0x3fffull;
+  return addr | (1ull << 16) | (32ull << 32) | (1ull << 46) | (4ull << 61);
+}
 // Bits of the instruction descriptor that say "A (B) is MN-major".
 constexpr uint32_t kIdescTransA = 1u << 15, kIdescTransB = 1u << 16;
 // Instruction descriptor: fp32 accumulate, bf16 A and B, both K-major, dense, N and M of the tile.

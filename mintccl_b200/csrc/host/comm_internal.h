@@ -55,7 +55,9 @@ int fail(const std::string& m);
 void* driver_entry(const char* name);
 // TMA descriptor of a row-major [rows, K] bf16 matrix cut into box_rows x 64 tiles (128-byte swizzle).
 int make_bf16_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t K, uint32_t box_rows);
-// The same for a matrix of bytes whose rows are `pitch` bytes apart (a multiple of 16): boxes of box_rows x 128.
-int make_u8_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t pitch, uint32_t box_rows);
+// The same for a matrix of bytes whose rows are `pitch` bytes apart (a multiple of 16): boxes of box_rows x box_cols
+// with the swizzle of that width (64 or 128).
+int make_u8_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t pitch, uint32_t box_rows,
+                uint32_t box_cols = 128);
 int sm_count(int device);
 }  // namespace mthost

@@ -3,6 +3,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <string.h>
+#include <stdlib.h>
 
 #include <string>
 
@@ -161,15 +162,16 @@ int mt_gemm_fp8(void* stream, const void* A, int64_t lda, const void* sa, int64_
     int dev = 0;
     cudaGetDevice(&dev);
     const int sms = nctas > 0 ? nctas : mthost::sm_count(dev);
-    const bool pair = M > 128 && sms > 1 && (M + 255) / 256 * ((N + 255) / 256) * 4 >= sms;
-    const int bn = pair ? 256 : 128, bm = pair ? 256 : 128;
+    const char* e1 = getenv("FP8_PAIR"); const char* e2 = getenv("FP8_BN");
+    const bool pair = e1 ? atoi(e1) : M > 128 && sms > 1 && (M + 255) / 256 * ((N + 127) / 128) * 4 >= sms;
+    const int bn = e2 ? atoi(e2) : 128, bm = pair ? 256 : 128;
     const int64_t tiles = (M + bm - 1) / bm * ((N + bn - 1) / bn);
     if (tiles > 0x3fffffffll) return fail("GEMM shape: too many tiles");
     mt::Fp8GemmArgs a;
     memset(&a, 0, sizeof(a));
     // K-major: boxes of 128 K x the tile's rows; stored transposed: 128 columns x 128 K rows
     if (ta ? mthost::make_u8_map(&a.a, A, K, M, lda, 128) : mthost::make_u8_map(&a.a, A, M, K, lda, 128)) return -1;
-    if (tb ? mthost::make_u8_map(&a.b, B, K, N, ldb, 128) : mthost::make_u8_map(&a.b, B, N, K, ldb, pair ? bn / 2 : bn)) return -1;
+    if (tb ? mthost::make_u8_map(&a.b, B, K, N, ldb, 128, pair ? bn / 2 : bn) : mthost::make_u8_map(&a.b, B, N, K, ldb, pair ? bn / 2 : bn)) return -1;
     a.sa = (const float*)sa;
     a.sb = (const float*)sb;
     a.sa_m = sa_m;

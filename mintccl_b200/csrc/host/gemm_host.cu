@@ -99,16 +99,17 @@ namespace mthost {
 int make_bf16_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t K, uint32_t box_rows) {
   return make_map(map, base, rows, K, box_rows);
 }
-int make_u8_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t pitch, uint32_t box_rows) {
+int make_u8_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t pitch, uint32_t box_rows,
+                uint32_t box_cols) {
   static EncodeTiledFn enc = (EncodeTiledFn)driver_entry("cuTensorMapEncodeTiled");
   if (!enc) return fail("cuTensorMapEncodeTiled not available");
   if (((uintptr_t)base & 15) || pitch % 16) return fail("8-bit operands must be 16-byte aligned with rows a multiple of 16 bytes apart");
   cuuint64_t dims[2] = {cols, rows};
   cuuint64_t strides[1] = {pitch};
-  cuuint32_t box[2] = {128, box_rows};
+  cuuint32_t box[2] = {box_cols, box_rows};
   cuuint32_t estr[2] = {1, 1};
   CUresult r = with_context([&] { return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, (void*)base, dims, strides, box, estr,
-                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE); });
   if (r != CUDA_SUCCESS) return fail("cuTensorMapEncodeTiled (bytes) failed: CUresult " + std::to_string((int)r));
   return 0;

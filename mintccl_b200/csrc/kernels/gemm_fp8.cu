@@ -47,15 +47,15 @@ template <int BN, bool PAIR>
 struct Shape {
   static constexpr int BNC = PAIR ? BN / 2 : BN;          // rows of B staged by a CTA
   static constexpr uint32_t B_BYTES = BNC * BK;
-  static constexpr int STAGES = A_BYTES + B_BYTES > 40000 ? 3 : 5;
-  static constexpr int ACC = BN > 128 ? 2 : 4;            // accumulators in TMEM
+  static constexpr int STAGES = PAIR ? 7 : 5;
+  static constexpr int ACC = TMEM_COLS / BN;              // accumulators
   static constexpr uint32_t OPERANDS = STAGES * (A_BYTES + B_BYTES);
   static constexpr uint32_t RING = kScaleSlots * 2 * BM * 4, STAGING = kSumWarps * 32 * kPitch;
   static constexpr uint32_t SMEM = 1024 + OPERANDS + RING + STAGING + 256;
   static_assert(SMEM <= 232448, "shared memory of one CTA");
 };
 struct Ctl {
-  uint64_t full[5], empty[5], acc_full[4], acc_empty[4], drain;
+  uint64_t full[7], empty[7], acc_full[4], acc_empty[4], drain;
   uint32_t tmem_base;
   int abort;
 };
@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_fp8_kernel(const __grid_cons
   constexpr int STAGES = S::STAGES, ACC = S::ACC, BNC = S::BNC, CW = BN / 2;   // CW: columns of a sum thread
   constexpr uint32_t B_BYTES = S::B_BYTES;
   constexpr int kRows = PAIR ? 2 * BM : BM;   // of a tile
-  static_assert(!TB || BNC % 128 == 0, "an operand stored transposed comes in chunks of 128 columns");
+  static_assert(BNC == 128 || BNC == 64, "columns of B that a CTA stages: one chunk");
   extern __shared__ uint8_t smem_raw[];
   // the same offsets in both CTAs: the MMA descriptors name shared memory of the pair by offset
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -218,12 +218,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_fp8_kernel(const __grid_cons
             if (cr == 0) mbar_expect_tx(&ctl->full[s], (PAIR ? 2 : 1) * (A_BYTES + B_BYTES));
             if (TA) load(sA + s * A_BYTES, &a.a, arow, kb * BK);
             else load(sA + s * A_BYTES, &a.a, kb * BK, arow);
-            if (TB) {
-#pragma unroll
-              for (int c = 0; c < BNC / 128; ++c) load(sB + s * B_BYTES + c * (128 * BK), &a.b, brow + c * 128, kb * BK);
-            } else {
-              load(sB + s * B_BYTES, &a.b, kb * BK, brow);
-            }
+            if (TB) load(sB + s * B_BYTES, &a.b, brow, kb * BK);
+            else load(sB + s * B_BYTES, &a.b, kb * BK, brow);
           }
           __syncwarp();
           s = sn;
@@ -239,7 +235,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_fp8_kernel(const __grid_cons
       // ---------------------------------------------------------- MMA issuer: uniform, one lane issues
       constexpr uint32_t idesc = make_idesc_e4m3(kRows, BN) | (TA ? kIdescTransA : 0u) | (TB ? kIdescTransB : 0u);
       // a step of 32 along K: 32 bytes of a row, or 32 rows of 128 bytes
-      constexpr uint64_t step_a = TA ? 256 : 2, step_b = TB ? 256 : 2;
+      constexpr uint64_t step_a = TA ? 256 : 2, step_b = !TB ? 2 : BNC == 128 ? 256 : 128;
       uint32_t s = 0, ph = 0, b = 0, bph = 0;
       bool ok = true;
       auto commit = [&](uint64_t* bar) {
@@ -258,7 +254,9 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_fp8_kernel(const __grid_cons
           }
           tc_fence_after();
           const uint64_t da = TA ? make_smem_desc_mn_sw128(sA + s * A_BYTES, 128 * BK) : make_smem_desc_sw128(sA + s * A_BYTES);
-          const uint64_t db = TB ? make_smem_desc_mn_sw128(sB + s * B_BYTES, 128 * BK) : make_smem_desc_sw128(sB + s * B_BYTES);
+          const uint64_t db = !TB          ? make_smem_desc_sw128(sB + s * B_BYTES)
+                              : BNC == 128 ? make_smem_desc_mn_sw128(sB + s * B_BYTES, 128 * BK)
+                                           : make_smem_desc_mn_sw64(sB + s * B_BYTES);
           if (elect_one()) {
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
@@ -362,31 +360,26 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_fp8_kernel(const __grid_cons
         }
         __syncwarp();
         tc_fence_after();
-        // 16 columns at a time: the next ones arrive while these are added, and the accumulator goes back to the tensor
-        // core before the last are
+        // all columns to registers, and the accumulator back to the tensor core before they are added
         const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + b * BN + half * CW;
         const uint32_t bn = b + 1 == ACC ? 0 : b + 1, bphn = b + 1 == ACC ? bph ^ 1 : bph;
-        uint32_t r[2][16];
-        tmem_ld_32x16(taddr, r[0]);
+        uint32_t r[CW / 32][32];
+#pragma unroll
+        for (int c = 0; c < CW / 32; ++c) tmem_ld_32x32(taddr + c * 32, r[c]);
         const uint32_t f = __float_as_uint(factor[(pos++ & (kScaleSlots - 1)) * (2 * BM)]);
         const uint64_t f2 = pack2(f, f);
-#pragma unroll
-        for (int c = 0; c < CW / 16; ++c) {
-          tmem_ld_wait();
-          if (c == CW / 16 - 3) ready = mbar_test(&ctl->acc_full[bn], bphn);   // known by the time it is needed
-          if (c + 1 < CW / 16) {
-            tmem_ld_32x16(taddr + (c + 1) * 16, r[(c + 1) & 1]);
-          } else {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) {
-              if (PAIR) mbar_arrive_cluster(empty_leader + b * 8);
-              else mbar_arrive(&ctl->acc_empty[b]);
-            }
-          }
-#pragma unroll
-          for (int i = 0; i < 8; ++i) fma2(acc[c * 8 + i], pack2(r[c & 1][2 * i], r[c & 1][2 * i + 1]), f2);
+        tmem_ld_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (PAIR) mbar_arrive_cluster(empty_leader + b * 8);
+          else mbar_arrive(&ctl->acc_empty[b]);
         }
+        ready = mbar_test(&ctl->acc_full[bn], bphn);   // known by the time it is needed
+#pragma unroll
+        for (int c = 0; c < CW / 32; ++c)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) fma2(acc[c * 16 + i], pack2(r[c][2 * i], r[c][2 * i + 1]), f2);
         b = bn;
         bph = bphn;
       }
@@ -449,8 +442,7 @@ cudaError_t go_form(bool ta, bool tb, const Fp8GemmArgs& a, int nctas, cudaStrea
 cudaError_t launch_fp8_gemm(int bn, bool pair, bool ta, bool tb, const Fp8GemmArgs& a, int nctas, cudaStream_t s) {
   if (ta && !tb) return cudaErrorInvalidValue;
   count_launch();
-  if (pair && bn == 256) return fp8g::go_form<256, true>(ta, tb, a, nctas, s);
-  if (!pair && bn == 128) return fp8g::go_form<128, false>(ta, tb, a, nctas, s);
+  if (bn == 128) return pair ? fp8g::go_form<128, true>(ta, tb, a, nctas, s) : fp8g::go_form<128, false>(ta, tb, a, nctas, s);
   return cudaErrorInvalidValue;
 }
 
