@@ -85,59 +85,49 @@ __device__ __forceinline__ void tile_of(int t, int mt_, int nt, int* mb, int* nb
   *mb = gr * 16 + in - *nb * rows;
 }
 
-// The sums of a warp's 32 rows and CW columns to C.  Whole aligned rows go through shared memory, 128 bytes of every row at
-// a time, so that stores are whole lines; otherwise by elements.
+// The sums of a warp's 32 rows and CW columns to C, 128 bytes of every row at a time through shared memory, so that stores
+// are whole lines: 16 bytes a lane where C's rows are aligned to that, else neighbouring elements on neighbouring lanes.
 template <class T, int CW>
 __device__ __forceinline__ void store_sums(const Fp8GemmArgs& a, const uint64_t* acc, uint8_t* stg, int row0, int col, int lane) {
   using E = typename T::elem;
-  constexpr int kE = (int)sizeof(E), kPer = 128 / kE, kRounds = (CW + kPer - 1) / kPer;   // columns of a round
-  const int n = a.N - col, rows = a.M - row0;   // may exceed the warp's part
+  constexpr int kE = (int)sizeof(E), kPer = 128 / kE;   // columns of a round
+  static_assert(CW % kPer == 0, "whole rounds");
+  const int n = min(CW, a.N - col), rows = min(32, a.M - row0);
   uint8_t* base = (uint8_t*)a.c + ((int64_t)row0 * a.ldc + col) * kE;
-  if (a.vec_out && n >= CW) {
 #pragma unroll
-    for (int r = 0; r < kRounds; ++r) {
-      constexpr int kTail = CW % kPer;
-      const int cols = r == kRounds - 1 && kTail ? kTail : kPer;
-      uint4* mine = (uint4*)(stg + lane * kPitch);
+  for (int r = 0; r < CW / kPer; ++r) {
+    uint4* mine = (uint4*)(stg + lane * kPitch);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (j * 16 < cols * kE) {
-          uint32_t w[4];
-          float f[16 / kE];
+    for (int j = 0; j < 8; ++j) {
+      float f[16 / kE];
 #pragma unroll
-          for (int i = 0; i < 8 / kE; ++i) {
-            const float2 x = unpack2(acc[(r * kPer + j * 16 / kE) / 2 + i]);
-            f[2 * i] = x.x;
-            f[2 * i + 1] = x.y;
-          }
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const uint64_t v = T::pack(f + i * T::kPer64);
-            w[2 * i] = (uint32_t)v;
-            w[2 * i + 1] = (uint32_t)(v >> 32);
-          }
-          mine[j] = make_uint4(w[0], w[1], w[2], w[3]);
-        }
+      for (int i = 0; i < 8 / kE; ++i) {
+        const float2 x = unpack2(acc[(r * kPer + j * 16 / kE) / 2 + i]);
+        f[2 * i] = x.x;
+        f[2 * i + 1] = x.y;
       }
-      __syncwarp();
+      const uint64_t lo = T::pack(f), hi = T::pack(f + T::kPer64);
+      mine[j] = make_uint4((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
+    }
+    __syncwarp();
+    if (a.vec_out && n == CW) {
       const int c16 = lane & 7;
-      if (c16 * 16 < cols * kE) {
 #pragma unroll
-        for (int p = 0; p < 8; ++p) {
-          const int rr = p * 4 + (lane >> 3);
-          if (rr < rows) *(uint4*)(base + ((int64_t)rr * a.ldc + r * kPer) * kE + c16 * 16) = *(const uint4*)(stg + rr * kPitch + c16 * 16);
-        }
+      for (int p = 0; p < 8; ++p) {
+        const int rr = p * 4 + (lane >> 3);
+        if (rr < rows) *(uint4*)(base + ((int64_t)rr * a.ldc + r * kPer) * kE + c16 * 16) = *(const uint4*)(stg + rr * kPitch + c16 * 16);
       }
-      __syncwarp();
-    }
-  } else if (lane < rows) {
-    E* e = (E*)base + (int64_t)lane * a.ldc;
+    } else {
+      E* to = (E*)base + r * kPer + lane;
+#pragma unroll 4
+      for (int rr = 0; rr < rows; ++rr, to += a.ldc) {
+        const E* from = (const E*)(stg + rr * kPitch) + lane;
 #pragma unroll
-    for (int i = 0; i < CW / 2; ++i) {
-      const float2 x = unpack2(acc[i]);
-      if (2 * i < n) e[2 * i] = float_to_elem<T>(x.x);
-      if (2 * i + 1 < n) e[2 * i + 1] = float_to_elem<T>(x.y);
+        for (int i = 0; i < kPer; i += 32)
+          if (r * kPer + i + lane < n) to[i] = from[i];
+      }
     }
+    __syncwarp();
   }
 }
 
