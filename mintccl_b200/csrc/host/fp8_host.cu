@@ -3,7 +3,6 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <string.h>
-#include <stdlib.h>
 
 #include <string>
 
@@ -162,16 +161,21 @@ int mt_gemm_fp8(void* stream, const void* A, int64_t lda, const void* sa, int64_
     int dev = 0;
     cudaGetDevice(&dev);
     const int sms = nctas > 0 ? nctas : mthost::sm_count(dev);
-    const char* e1 = getenv("FP8_PAIR"); const char* e2 = getenv("FP8_BN");
-    const bool pair = e1 ? atoi(e1) : M > 128 && sms > 1 && (M + 255) / 256 * ((N + 127) / 128) * 4 >= sms;
-    const int bn = e2 ? atoi(e2) : 128, bm = pair ? 256 : 128;
-    const int64_t tiles = (M + bm - 1) / bm * ((N + bn - 1) / bn);
+    // Pairs where single CTAs would need more than one wave.  Fewer tiles than half the SMs: CTAs share a tile along K, at
+    // least eight blocks each; adding up and the skew of the CTAs cost about 2 us, a block 0.25.  Measured (us, 1 / 2 / 4 / 8
+    // CTAs a tile): 1 x 4096 x 4096 12.6 / 10.2 / 8.9, 128 x 1024 x 8192 21.3 / 15.5 / 11.5 / 10.2, 64 x 64 x 8192 22.1 / 15.4 /
+    // 10.6 / 8.1, 1001 x 1111 x 2050 13.0 / 11.0; 128 x 4096 x 1792 (14 blocks) 8.6 / 9.3 / 9.0.
+    const int64_t nt = (N + 127) / 128, singles = (M + 127) / 128 * nt, blocks = (K + 127) / 128;
+    const bool pair = M > 128 && sms > 1 && singles > sms;
+    const int64_t tiles = pair ? (M + 255) / 256 * nt : singles;
+    int split = 1;
+    while (!pair && split < 8 && tiles * split * 2 <= sms && split * 16 <= blocks) split *= 2;
     if (tiles > 0x3fffffffll) return fail("GEMM shape: too many tiles");
     mt::Fp8GemmArgs a;
     memset(&a, 0, sizeof(a));
-    // K-major: boxes of 128 K x the tile's rows; stored transposed: 128 columns x 128 K rows
+    // K-major: boxes of 128 K x the CTA's rows; stored transposed: its columns x 128 K rows
     if (ta ? mthost::make_u8_map(&a.a, A, K, M, lda, 128) : mthost::make_u8_map(&a.a, A, M, K, lda, 128)) return -1;
-    if (tb ? mthost::make_u8_map(&a.b, B, K, N, ldb, 128, pair ? bn / 2 : bn) : mthost::make_u8_map(&a.b, B, N, K, ldb, pair ? bn / 2 : bn)) return -1;
+    if (tb ? mthost::make_u8_map(&a.b, B, K, N, ldb, 128, pair ? 64 : 128) : mthost::make_u8_map(&a.b, B, N, K, ldb, pair ? 64 : 128)) return -1;
     a.sa = (const float*)sa;
     a.sb = (const float*)sb;
     a.sa_m = sa_m;
@@ -187,7 +191,8 @@ int mt_gemm_fp8(void* stream, const void* A, int64_t lda, const void* sa, int64_
     a.vec_out = vec_of(C, ldc, elem_size(dtype)) > 0;
     a.timeout_ns = 4000000000ull;
     const int units = pair ? sms / 2 : sms, used = (int)(tiles < units ? tiles : units);
-    if (launched(mt::launch_fp8_gemm(bn, pair, ta != 0, tb != 0, a, pair ? 2 * used : used, (cudaStream_t)stream), "fp8 gemm"))
+    const int grid = pair ? 2 * used : split > 1 ? split * (int)tiles : used;
+    if (launched(mt::launch_fp8_gemm(pair, split, ta != 0, tb != 0, a, grid, (cudaStream_t)stream), "fp8 gemm"))
       return -1;
     mthost::stat_add(mthost::ST_GEMM, (uint64_t)(2.0 * M * N * K));
     return 0;

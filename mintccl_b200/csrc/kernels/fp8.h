@@ -58,8 +58,9 @@ struct Fp8GemmArgs {
   int32_t vec_out;                  // rows of C start on 16-byte boundaries
   uint64_t timeout_ns;
 };
-// bn: columns of a tile; pair: tiles of 256 rows on CTA pairs (nctas even), else of 128
-cudaError_t launch_fp8_gemm(int bn, bool pair, bool ta, bool tb, const Fp8GemmArgs& a, int nctas, cudaStream_t s);
+// Tiles of 128 columns.  pair: 256 rows each, on CTA pairs (nctas even).  Else 128 rows each; split (1, 2, 4 or 8): the
+// CTAs that share a tile's blocks along K, at most as many as there are blocks; nctas = split * tiles if it is not 1.
+cudaError_t launch_fp8_gemm(bool pair, int split, bool ta, bool tb, const Fp8GemmArgs& a, int nctas, cudaStream_t s);
 int fp8_gemm_error();   // 1 after a wait of the kernel expired (synchronises), -1 on a CUDA error
 
 }  // namespace mt

@@ -11,6 +11,11 @@
 // PAIR: two CTAs of a cluster share one tile of 256 rows (cta_group::2), each with its 128 rows of A, half of the tile's
 // rows of B and its half of the accumulator; the leader (cluster rank 0) issues for both.
 //
+// Without PAIR a tile of 128 rows is one CTA's, or that of a cluster of up to eight which share out the blocks along K
+// (few tiles, so that the others of the chip's SMs load and multiply too).  Each then leaves its sums in its shared memory
+// and adds up its share of the tile's rows from all of them, in the order of the blocks: the same bits every time.  (Sending
+// them instead, with stores or bulk copies to the other CTAs' shared memory, took 1 - 2 us longer for 128 rows.)
+//
 //   warps 0..7   sums: a thread has one row and half of the tile's columns; then they store C
 //   warp 8       TMA producer: own halves of A and B; the bytes of both CTAs count on the leader's "stage full" barrier
 //   warp 9       (leader) issues tcgen05.mma: four a stage; commits to "stage empty" and "accumulator full" of both CTAs
@@ -41,6 +46,7 @@ constexpr int kRegsSum = 224, kRegsRest = 56, kRegsLaunch = 168;
 static_assert(kRegsSum * kSumThreads + kRegsRest * 128 <= kRegsLaunch * kThreads, "registers of the CTA");
 constexpr int kScaleSlots = 16;     // blocks whose scales wait in shared memory
 constexpr int kPitch = 144;         // bytes of a staged row of C: 128 and padding
+constexpr int kSumPitch = 132;      // floats of a row of sums in shared memory
 constexpr uint32_t A_BYTES = BM * BK, TMEM_COLS = 512;
 
 template <int BN, bool PAIR>
@@ -53,6 +59,7 @@ struct Shape {
   static constexpr uint32_t RING = kScaleSlots * 2 * BM * 4, STAGING = kSumWarps * 32 * kPitch;
   static constexpr uint32_t SMEM = 1024 + OPERANDS + RING + STAGING + 256;
   static_assert(SMEM <= 232448, "shared memory of one CTA");
+  static_assert(PAIR || OPERANDS >= BM * kSumPitch * 4, "the sums of a split tile are left where the stages were");
 };
 struct Ctl {
   uint64_t full[7], empty[7], acc_full[4], acc_empty[4], drain;
@@ -131,6 +138,47 @@ __device__ __forceinline__ void store_sums(const Fp8GemmArgs& a, const uint64_t*
   }
 }
 
+// This CTA's share of a split tile's rows to C: the sums of all CTAs of the cluster, four columns a thread, two rows' loads
+// in flight.
+template <class T, int SPLIT>
+__device__ __forceinline__ void store_split(const Fp8GemmArgs& a, uint32_t sums, int rank, int row0, int col0) {
+  using E = typename T::elem;
+  constexpr int kRowsEach = BM / SPLIT;
+  const int c = (threadIdx.x & 31) * 4, n = a.N - (col0 + c);
+  if (n <= 0) return;
+#pragma unroll 2
+  for (int i = threadIdx.x >> 5; i < kRowsEach; i += kSumWarps) {
+    const int r = rank * kRowsEach + i, row = row0 + r;
+    if (row >= a.M) break;
+    float4 x[SPLIT];
+#pragma unroll
+    for (int s = 0; s < SPLIT; ++s) x[s] = ld_cluster_f4(map_to_cta(sums + (r * kSumPitch + c) * 4, s));
+    float f[4] = {x[0].x, x[0].y, x[0].z, x[0].w};
+#pragma unroll
+    for (int s = 1; s < SPLIT; ++s) {
+      f[0] += x[s].x;
+      f[1] += x[s].y;
+      f[2] += x[s].z;
+      f[3] += x[s].w;
+    }
+    E* to = (E*)a.c + (int64_t)row * a.ldc + col0 + c;
+    if (a.vec_out && n >= 4) {
+      if constexpr (sizeof(E) == 4) *(float4*)to = make_float4(f[0], f[1], f[2], f[3]);
+      else *(uint64_t*)to = T::pack(f);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j < n) to[j] = float_to_elem<T>(f[j]);
+    }
+  }
+}
+template <class T>
+__device__ __forceinline__ void store_split(const Fp8GemmArgs& a, uint32_t sums, int split, int rank, int row0, int col0) {
+  if (split == 2) store_split<T, 2>(a, sums, rank, row0, col0);
+  else if (split == 4) store_split<T, 4>(a, sums, rank, row0, col0);
+  else store_split<T, 8>(a, sums, rank, row0, col0);
+}
+
 template <int BN, bool PAIR, bool TA, bool TB>
 __global__ void __launch_bounds__(kThreads, 1) gemm_fp8_kernel(const __grid_constant__ Fp8GemmArgs a) {
   using S = Shape<BN, PAIR>;
@@ -149,20 +197,48 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_fp8_kernel(const __grid_cons
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const int cr = PAIR ? (int)cluster_ctarank() : 0;
 
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&ctl->full[s], PAIR ? 3 : 2);   // the producer's byte count and the scales of each CTA
-      mbar_init(&ctl->empty[s], 1);
+  const int mt_ = (a.M + kRows - 1) / kRows, nt = (a.N + BN - 1) / BN, tiles = mt_ * nt, allblocks = (a.K + BK - 1) / BK;
+  // a split tile is the only one of its cluster
+  const int split = PAIR ? 1 : (int)cluster_nctas(), share = PAIR ? 0 : (int)cluster_ctarank();
+  const int group = PAIR ? 2 : split, first = (int)blockIdx.x / group, step = (int)gridDim.x / group;
+  const int kfirst = allblocks * share / split, kblocks = allblocks * (share + 1) / split - kfirst;
+
+  // one stage of tile (mb, nb), by one thread
+  auto load_stage = [&](uint32_t s, int mb, int nb, int kb) {
+    const int arow = mb * kRows + cr * BM, brow = nb * BN + cr * BNC, k = (kfirst + kb) * BK;
+    const uint32_t full = PAIR ? map_to_cta(smem_u32(&ctl->full[s]), 0) : 0;
+    auto load = [&](uint8_t* dst, const CUtensorMap* map, int x, int y) {
+      if (PAIR) tma_load_2d_pair(dst, map, x, y, full);
+      else tma_load_2d(dst, map, x, y, &ctl->full[s]);
+    };
+    if (cr == 0) mbar_expect_tx(&ctl->full[s], (PAIR ? 2 : 1) * (A_BYTES + B_BYTES));
+    if (TA) load(sA + s * A_BYTES, &a.a, arow, k);
+    else load(sA + s * A_BYTES, &a.a, k, arow);
+    if (TB) load(sB + s * B_BYTES, &a.b, brow, k);
+    else load(sB + s * B_BYTES, &a.b, k, brow);
+  };
+  // the first tile's stages that need not wait for anything (a pair has to meet first)
+  const int early = PAIR || first >= tiles ? 0 : min(STAGES, kblocks);
+  if (warp == kSumWarps) {
+    if (elect_one()) {
+      for (int s = 0; s < STAGES; ++s) {
+        mbar_init(&ctl->full[s], PAIR ? 3 : 2);   // the producer's byte count and the scales of each CTA
+        mbar_init(&ctl->empty[s], 1);
+      }
+      for (int s = 0; s < ACC; ++s) {
+        mbar_init(&ctl->acc_full[s], 1);
+        mbar_init(&ctl->acc_empty[s], PAIR ? 2 * kSumWarps : kSumWarps);   // the leader's counts both CTAs
+      }
+      mbar_init(&ctl->drain, 1);
+      ctl->abort = 0;
+      fence_barrier_init();
+      if (early) {
+        int mb, nb;
+        tile_of(first, mt_, nt, &mb, &nb);
+        for (int s = 0; s < early; ++s) load_stage(s, mb, nb, s);
+      }
     }
-    for (int s = 0; s < ACC; ++s) {
-      mbar_init(&ctl->acc_full[s], 1);
-      mbar_init(&ctl->acc_empty[s], PAIR ? 2 * kSumWarps : kSumWarps);   // the leader's counts both CTAs
-    }
-    mbar_init(&ctl->drain, 1);
-    ctl->abort = 0;
-    fence_barrier_init();
-    tma_prefetch_desc(&a.a);
-    tma_prefetch_desc(&a.b);
+    __syncwarp();
   }
   if (warp == kSumWarps + 1) {
     if (PAIR) {
@@ -179,38 +255,24 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_fp8_kernel(const __grid_cons
   tc_fence_after();
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, ctl->tmem_base, 0);
   volatile int* abort_flag = &ctl->abort;
-  const int mt_ = (a.M + kRows - 1) / kRows, nt = (a.N + BN - 1) / BN, tiles = mt_ * nt, kblocks = (a.K + BK - 1) / BK;
-  const int first = PAIR ? blockIdx.x >> 1 : blockIdx.x, step = PAIR ? gridDim.x >> 1 : gridDim.x;
 
   if (warp >= kSumWarps) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsRest));
     if (warp == kSumWarps) {
       // ---------------------------------------------------------- TMA producer: a uniform warp, one lane issues
-      const uint32_t full_leader = map_to_cta(smem_u32(&ctl->full[0]), 0);
-      uint32_t s = 0, ph = 0;
-      bool ok = true, free = true;   // free: a probe found the next stage empty
-      auto load = [&](uint8_t* dst, const CUtensorMap* map, int x, int y) {
-        if (PAIR) tma_load_2d_pair(dst, map, x, y, full_leader + s * 8);
-        else tma_load_2d(dst, map, x, y, &ctl->full[s]);
-      };
+      uint32_t s = early == STAGES ? 0 : early, ph = early == STAGES;
+      bool ok = true, free = early < STAGES;   // free: a probe found the next stage empty
       for (int t = first; ok && t < tiles; t += step) {
         int mb, nb;
         tile_of(t, mt_, nt, &mb, &nb);
-        const int arow = mb * kRows + cr * BM, brow = nb * BN + cr * BNC;
-        for (int kb = 0; kb < kblocks; ++kb) {
+        for (int kb = t == first ? early : 0; kb < kblocks; ++kb) {
           if (!free && !wait_bar_warp(&ctl->empty[s], ph ^ 1, abort_flag, a.timeout_ns)) {
             ok = false;
             break;
           }
           const uint32_t sn = s + 1 == STAGES ? 0 : s + 1, phn = s + 1 == STAGES ? ph ^ 1 : ph;
           free = __all_sync(0xffffffffu, mbar_test(&ctl->empty[sn], phn ^ 1));
-          if (elect_one()) {
-            if (cr == 0) mbar_expect_tx(&ctl->full[s], (PAIR ? 2 : 1) * (A_BYTES + B_BYTES));
-            if (TA) load(sA + s * A_BYTES, &a.a, arow, kb * BK);
-            else load(sA + s * A_BYTES, &a.a, kb * BK, arow);
-            if (TB) load(sB + s * B_BYTES, &a.b, brow, kb * BK);
-            else load(sB + s * B_BYTES, &a.b, kb * BK, brow);
-          }
+          if (elect_one()) load_stage(s, mb, nb, kb);
           __syncwarp();
           s = sn;
           ph = phn;
@@ -289,9 +351,9 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_fp8_kernel(const __grid_cons
         const int row = mb * kRows + cr * BM + lane, c0 = nb * BN, c1 = c0 + CW;
         const float* pa[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) pa[i] = a.sa + (int64_t)(row + 32 * i < a.M ? row + 32 * i : 0) * a.sa_m;
-        const float* pb0 = a.sb + (int64_t)(c0 >> 7) * a.sb_n;
-        const float* pb1 = a.sb + (int64_t)(c1 < a.N ? c1 >> 7 : 0) * a.sb_n;
+        for (int i = 0; i < 4; ++i) pa[i] = a.sa + (int64_t)(row + 32 * i < a.M ? row + 32 * i : 0) * a.sa_m + kfirst * a.sa_k;
+        const float* pb0 = a.sb + (int64_t)(c0 >> 7) * a.sb_n + kfirst * a.sb_k;
+        const float* pb1 = a.sb + (int64_t)(c1 < a.N ? c1 >> 7 : 0) * a.sb_n + kfirst * a.sb_k;
         for (int kb = (pos + w) & 1; ok && kb < kblocks; kb += 4) {
           float va[2][4], vb[2][2];
 #pragma unroll
@@ -325,6 +387,10 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_fp8_kernel(const __grid_cons
           }
         }
       }
+    }
+    if (!PAIR && split > 1) {   // as the sum warps do
+      cluster_sync_all();
+      cluster_sync_all();
     }
   } else {
     // ------------------------------------------------------------ sums and C
@@ -373,11 +439,30 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_fp8_kernel(const __grid_cons
         b = bn;
         bph = bphn;
       }
-      if (ok && work) {
+      if (!PAIR && split > 1) {
+        // all products have arrived: the stages are free
+        float* mine = (float*)smem + (q * 32 + lane) * kSumPitch + half * CW;
+#pragma unroll
+        for (int i = 0; i < CW / 4; ++i) {
+          const float2 x = unpack2(acc[2 * i]), y = unpack2(acc[2 * i + 1]);
+          *(float4*)(mine + 4 * i) = make_float4(x.x, x.y, y.x, y.y);
+        }
+      } else if (ok && work) {
         if (a.out_dtype == DT_F32) store_sums<F32, CW>(a, acc, stg, row0, col, lane);
         else if (a.out_dtype == DT_BF16) store_sums<BF16, CW>(a, acc, stg, row0, col, lane);
         else store_sums<F16, CW>(a, acc, stg, row0, col, lane);
       }
+    }
+    if (!PAIR && split > 1) {
+      int mb, nb;
+      tile_of(first, mt_, nt, &mb, &nb);
+      const uint32_t sums = smem_u32(smem);
+      cluster_sync_all();   // the sums of all are in place
+      if (a.out_dtype == DT_F32) store_split<F32>(a, sums, split, share, mb * BM, nb * BN);
+      else if (a.out_dtype == DT_BF16) store_split<BF16>(a, sums, split, share, mb * BM, nb * BN);
+      else store_split<F16>(a, sums, split, share, mb * BM, nb * BN);
+      __syncwarp();
+      cluster_sync_all();   // nobody leaves while its sums may still be read
     }
   }
 
@@ -397,7 +482,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_fp8_kernel(const __grid_cons
 }
 
 template <int BN, bool PAIR, bool TA, bool TB>
-cudaError_t go(const Fp8GemmArgs& a, int nctas, cudaStream_t s) {
+cudaError_t go(const Fp8GemmArgs& a, int cluster, int nctas, cudaStream_t s) {
   const void* fn = (const void*)gemm_fp8_kernel<BN, PAIR, TA, TB>;
   // the register split waits forever for registers that the launch did not bring
   static const int regs = [&] {
@@ -415,25 +500,24 @@ cudaError_t go(const Fp8GemmArgs& a, int nctas, cudaStream_t s) {
   cfg.stream = s;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = PAIR ? 2 : 1;
+  at[0].val.clusterDim.x = cluster;
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, gemm_fp8_kernel<BN, PAIR, TA, TB>, a);
 }
 template <int BN, bool PAIR>
-cudaError_t go_form(bool ta, bool tb, const Fp8GemmArgs& a, int nctas, cudaStream_t s) {
-  if (ta) return go<BN, PAIR, true, true>(a, nctas, s);
-  return tb ? go<BN, PAIR, false, true>(a, nctas, s) : go<BN, PAIR, false, false>(a, nctas, s);
+cudaError_t go_form(bool ta, bool tb, const Fp8GemmArgs& a, int cluster, int nctas, cudaStream_t s) {
+  if (ta) return go<BN, PAIR, true, true>(a, cluster, nctas, s);
+  return tb ? go<BN, PAIR, false, true>(a, cluster, nctas, s) : go<BN, PAIR, false, false>(a, cluster, nctas, s);
 }
 
 }  // namespace fp8g
 
-cudaError_t launch_fp8_gemm(int bn, bool pair, bool ta, bool tb, const Fp8GemmArgs& a, int nctas, cudaStream_t s) {
-  if (ta && !tb) return cudaErrorInvalidValue;
+cudaError_t launch_fp8_gemm(bool pair, int split, bool ta, bool tb, const Fp8GemmArgs& a, int nctas, cudaStream_t s) {
+  if ((ta && !tb) || split < 1 || (pair && split > 1)) return cudaErrorInvalidValue;
   count_launch();
-  if (bn == 128) return pair ? fp8g::go_form<128, true>(ta, tb, a, nctas, s) : fp8g::go_form<128, false>(ta, tb, a, nctas, s);
-  return cudaErrorInvalidValue;
+  return pair ? fp8g::go_form<128, true>(ta, tb, a, 2, nctas, s) : fp8g::go_form<128, false>(ta, tb, a, split, nctas, s);
 }
 
 int fp8_gemm_error() {
