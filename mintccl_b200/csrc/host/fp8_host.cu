@@ -4,6 +4,8 @@
 #include <cuda_runtime.h>
 #include <string.h>
 
+#include <atomic>
+
 #include <string>
 
 #include "../kernels/fp8.h"
@@ -34,6 +36,17 @@ int vec_of(const void* p, int64_t ld, int esz) {
   return bits % 32 == 0 ? 2 : bits % 16 == 0 ? 1 : 0;
 }
 int narrower(int a, int b) { return a < b ? a : b; }
+
+// SMs of the current device, asked for once.
+int sms_here() {
+  static std::atomic<int> known[64];
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev > 63) return mthost::sm_count(dev);
+  int n = known[dev].load(std::memory_order_relaxed);
+  if (!n) known[dev].store(n = mthost::sm_count(dev), std::memory_order_relaxed);
+  return n;
+}
 
 int check_matrix(int64_t rows, int64_t cols, int64_t ldq, int dtype) {
   if (rows <= 0 || cols <= 0) return fail("rows and columns must be positive");
@@ -158,9 +171,7 @@ int mt_gemm_fp8(void* stream, const void* A, int64_t lda, const void* sa, int64_
     if (ta && !tb) return fail("ta goes with tb");
     if (!A || !B || !sa || !sb || !C || !elem_size(dtype) || ldc < N) return fail("bad GEMM operands");
     if (lda < (ta ? M : K) || ldb < (tb ? N : K)) return fail("rows of an operand overlap");
-    int dev = 0;
-    cudaGetDevice(&dev);
-    const int sms = nctas > 0 ? nctas : mthost::sm_count(dev);
+    const int sms = nctas > 0 ? nctas : sms_here();
     // Pairs where single CTAs would need more than one wave.  Fewer tiles than half the SMs: CTAs share a tile along K, at
     // least eight blocks each; adding up and the skew of the CTAs cost about 2 us, a block 0.25.  Measured (us, 1 / 2 / 4 / 8
     // CTAs a tile): 1 x 4096 x 4096 12.6 / 10.2 / 8.9, 128 x 1024 x 8192 21.3 / 15.5 / 11.5 / 10.2, 64 x 64 x 8192 22.1 / 15.4 /
@@ -197,6 +208,45 @@ int mt_gemm_fp8(void* stream, const void* A, int64_t lda, const void* sa, int64_
     mthost::stat_add(mthost::ST_GEMM, (uint64_t)(2.0 * M * N * K));
     return 0;
   });
+}
+
+int mt_fp8_packed(void* stream, int op, const int64_t* v) {
+  if (!v) return fail("no arguments");
+  auto p = [&](int i) { return (void*)(uintptr_t)v[i]; };
+  switch (op) {
+    case MT_FP8_QUANTIZE:
+      return mt_fp8_quantize(stream, (int)v[0], p(1), v[2], v[3], v[4], v[5], p(6), p(7), p(8), p(9), p(10), p(11));
+    case MT_FP8_DEQUANTIZE:
+      return mt_fp8_dequantize(stream, (int)v[0], p(1), v[2], p(3), v[4], v[5], v[6], v[7], (int)v[8], (int)v[9], p(10), v[11]);
+    case MT_FP8_ACT_FORWARD:
+      return mt_fp8_act_forward(stream, (int)v[0], p(1), v[2], p(3), v[4], v[5], v[6], p(7), v[8], v[9], p(10), p(11), p(12), p(13));
+    case MT_FP8_ACT_BACKWARD:
+      return mt_fp8_act_backward(stream, (int)v[0], v[1], p(2), p(3), v[4], v[5], p(6), p(7), v[8], v[9], p(10), v[11], v[12], v[13],
+                                 p(14), p(15), p(16));
+    case MT_FP8_GEMM:
+      return mt_gemm_fp8(stream, p(0), v[1], p(2), v[3], v[4], p(5), v[6], p(7), v[8], v[9], p(10), v[11], (int)v[12], v[13], v[14],
+                         v[15], (int)v[16], (int)v[17], (int)v[18]);
+    case MT_FP8_LINEAR_FORWARD: {
+      const int64_t T = v[3], K = v[4], N = v[8], ldq = (K + 15) / 16 * 16;
+      if (mt_fp8_quantize(stream, (int)v[0], p(1), v[2], T, K, ldq, p(9), p(10), nullptr, nullptr, p(11), p(12))) return -1;
+      if (v[6] && mt_fp8_quantize(stream, (int)v[5], p(6), v[7], N, K, v[14], nullptr, nullptr, nullptr, nullptr, p(13), p(15))) return -1;
+      return mt_gemm_fp8(stream, p(9), ldq, p(10), 1, T, p(13), v[14], p(15), v[16], v[17], p(18), N, (int)v[0], T, N, K, 0, 0, 0);
+    }
+    case MT_FP8_LINEAR_BACKWARD: {
+      const int64_t T = v[3], N = v[4], K = v[5], ldq = (N + 15) / 16 * 16, ldx = (K + 15) / 16 * 16;
+      const bool want_x = v[13] != 0, want_w = v[18] != 0;
+      if (mt_fp8_quantize(stream, (int)v[0], p(1), v[2], T, N, ldq, want_x ? p(6) : nullptr, want_x ? p(7) : nullptr,
+                          want_w ? p(14) : nullptr, want_w ? p(15) : nullptr, nullptr, nullptr))
+        return -1;
+      if (want_x && mt_gemm_fp8(stream, p(6), ldq, p(7), 1, T, p(8), v[9], p(10), v[12], v[11], p(13), K, (int)v[0], T, K, N, 0, 1, 0))
+        return -1;
+      if (want_w && mt_gemm_fp8(stream, p(14), ldq, p(15), 1, N, p(16), ldx, p(17), 1, (K + 127) / 128, p(18), K, (int)v[19], N, K, T, 1,
+                                1, 0))
+        return -1;
+      return 0;
+    }
+    default: return fail("unknown operation");
+  }
 }
 
 int mt_gemm_fp8_error(void) { return mt::fp8_gemm_error(); }

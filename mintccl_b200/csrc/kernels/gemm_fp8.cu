@@ -28,6 +28,8 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
+
 #include "../device/prims.cuh"
 #include "../device/reduce_ops.cuh"
 #include "../device/tc_prims.cuh"
@@ -484,15 +486,18 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_fp8_kernel(const __grid_cons
 template <int BN, bool PAIR, bool TA, bool TB>
 cudaError_t go(const Fp8GemmArgs& a, int cluster, int nctas, cudaStream_t s) {
   const void* fn = (const void*)gemm_fp8_kernel<BN, PAIR, TA, TB>;
-  // the register split waits forever for registers that the launch did not bring
-  static const int regs = [&] {
-    cudaFuncAttributes at;
-    return cudaFuncGetAttributes(&at, fn) == cudaSuccess ? at.numRegs : 0;
-  }();
-  if (regs < kRegsLaunch) return cudaErrorLaunchOutOfResources;
-  // per device, and cheap enough to say at every launch
-  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<BN, PAIR>::SMEM);
+  static std::atomic<uint64_t> ready{0};   // devices on which the kernel has been looked over and given its shared memory
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (dev > 63 || !(ready.load(std::memory_order_acquire) & bit)) {
+    cudaFuncAttributes at;
+    if ((e = cudaFuncGetAttributes(&at, fn)) != cudaSuccess) return e;
+    if (at.numRegs < kRegsLaunch) return cudaErrorLaunchOutOfResources;   // the register split would wait forever for what is missing
+    if ((e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<BN, PAIR>::SMEM)) != cudaSuccess) return e;
+    if (dev <= 63) ready.fetch_or(bit, std::memory_order_release);
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(nctas);
   cfg.blockDim = dim3(kThreads);

@@ -178,6 +178,18 @@ int mt_fp8_act_backward(void* stream, int dtype, int64_t ldq, const void* h_data
 int mt_gemm_fp8(void* stream, const void* A, int64_t lda, const void* sa, int64_t sa_m, int64_t sa_k, const void* B, int64_t ldb,
                 const void* sb, int64_t sb_n, int64_t sb_k, void* C, int64_t ldc, int dtype, int64_t M, int64_t N, int64_t K,
                 int ta, int tb, int nctas);
+// The functions above with their arguments after `stream` as 64-bit integers (ctypes takes 3 us to convert twenty
+// arguments one by one), and the two passes of a linear layer, each of them all of its kernels in one call.
+//   MT_FP8_LINEAR_FORWARD   dtype, x, ldx, T, K, w_dtype, w (0: encoded already), ldw, N, xr_data, xr_scale, xt_data, xt_scale
+//                           (both 0: not wanted), w_data, ldwq, w_scale, w_srow, w_scol, y
+//       payloads of x are ceil16(K) bytes a row, xr and xt its row blocks and tiles; w's tiles are written if w is given;
+//       y [T, N] of x's dtype, contiguous
+//   MT_FP8_LINEAR_BACKWARD  dtype, dy, lddy, T, N, K, r_data, r_scale, w_data, ldwq, w_scale, w_srow, w_scol, dx (0: none),
+//                           c_data, c_scale, xt_data, xt_scale, dw (0: none), w_dtype
+//       r and c: room for the row and column blocks of dy [T, N], ceil16(N) bytes a row; dx [T, K] and dw [N, K] contiguous
+enum { MT_FP8_QUANTIZE = 0, MT_FP8_DEQUANTIZE, MT_FP8_ACT_FORWARD, MT_FP8_ACT_BACKWARD, MT_FP8_GEMM, MT_FP8_LINEAR_FORWARD,
+       MT_FP8_LINEAR_BACKWARD };
+int mt_fp8_packed(void* stream, int op, const int64_t* args);
 // 1 after a bounded wait of mt_gemm_fp8 expired (synchronises; the result of that call is then invalid), 0 otherwise
 int mt_gemm_fp8_error(void);
 

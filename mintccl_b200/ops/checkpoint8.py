@@ -15,10 +15,8 @@ from typing import NamedTuple, Optional, Tuple
 
 import torch
 
-from .. import _native as N
-from .fp8 import DTYPES, _cdiv, _check_float, _new_payload, _new_scale, _payload, _plain_scale, _row_stride, _rows, _scale_shape
-from .fp8 import dequantize_fp8, quantize_fp8
-from .mxfp8 import _on_device, _plain_cuda
+from .fp8 import ACT_BACKWARD, ACT_FORWARD, DTYPES, _call, _check_float, _check_scale, _native, _new_payload, _new_scale, _payload
+from .fp8 import _rows, _scale_shape, _up16, dequantize_fp8, quantize_fp8
 
 
 class Saved8(NamedTuple):
@@ -34,10 +32,13 @@ class Saved8(NamedTuple):
 
     def restore(self, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
         """The tensor again, contiguous, in its own type or ``dtype``."""
-        return dequantize_fp8(self.data, self.scale, "row", dtype or self.dtype).view(self.shape)
+        x = dequantize_fp8(self.data, self.scale, "row", dtype or self.dtype)
+        return x if len(self.shape) == 2 else x.view(self.shape)
 
 
 def _matrix(x: torch.Tensor) -> torch.Tensor:
+    if x.dim() == 2:
+        return x
     cols = x.shape[-1] if x.dim() else 1
     return x.reshape(x.numel() // cols if cols else 0, cols)
 
@@ -52,22 +53,27 @@ def _forward(h: torch.Tensor, u: Optional[torch.Tensor]):
     _check_float(h, "the input")
     if u is not None and (u.shape != h.shape or u.dtype != h.dtype or u.device != h.device):
         raise ValueError("gate and up must be of one shape, type and device")
-    h2, u2 = _matrix(h.detach()), None if u is None else _matrix(u.detach())
-    if not _plain_cuda(h2) or (u is not None and not _plain_cuda(u2)):
+    h2, u2 = _matrix(h), None if u is None else _matrix(u)
+    if not _native(*((h2,) if u is None else (h2, u2))):
         hf = h.detach().float()
         y = hf / (1 + torch.exp(-hf))
         y = (y if u is None else y * u.detach().float()).to(h.dtype)
         return y, save8(h), None if u is None else save8(u)
-    rows, cols = h2.shape
-    ins = [_rows(t) for t in (h2, u2) if t is not None]
-    kept = [(_new_payload(rows, cols, h.device), _new_scale(rows, cols, "row", h.device)) for _ in ins]
-    y = torch.empty(rows, cols, device=h.device, dtype=h.dtype)
+    (rows, cols), dev = h2.shape, h.device
+    hd, hs = _new_payload(rows, cols, dev), _new_scale(rows, cols, "row", dev)
+    y = torch.empty(h.shape, device=dev, dtype=h.dtype)
+    h2, ldh = _rows(h2)
+    if u is None:
+        ud = us = None
+        up = 0, 0, 0, 0
+    else:
+        ud, us = _new_payload(rows, cols, dev), _new_scale(rows, cols, "row", dev)
+        u2, ldu = _rows(u2)
+        up = u2.data_ptr(), ldu, ud.data_ptr(), us.data_ptr()
     if y.numel():
-        ptrs = [p for t in ins for p in (t.data_ptr(), _row_stride(t))] + ([None, 0] if u is None else [])
-        keep = [t.data_ptr() for k in kept for t in k] + ([None, None] if u is None else [])
-        _on_device(y, N.lib().mt_fp8_act_forward, DTYPES[h.dtype], *ptrs, rows, cols, y.data_ptr(), cols, _cdiv(cols, 16) * 16, *keep)
-    saved = [Saved8(*k, h.shape, h.dtype) for k in kept]
-    return y.view(h.shape), saved[0], None if u is None else saved[1]
+        _call(ACT_FORWARD, y.get_device(), DTYPES[h.dtype], h2.data_ptr(), ldh, up[0], up[1], rows, cols, y.data_ptr(), cols, _up16(cols),
+              hd.data_ptr(), hs.data_ptr(), up[2], up[3])
+    return y, Saved8(hd, hs, h.shape, h.dtype), None if u is None else Saved8(ud, us, h.shape, h.dtype)
 
 
 def _backward(h: Saved8, u: Optional[Saved8], dy: torch.Tensor, act: bool):
@@ -75,32 +81,35 @@ def _backward(h: Saved8, u: Optional[Saved8], dy: torch.Tensor, act: bool):
         raise ValueError("dy must have the shape, type and device of the activation")
     if u is not None and (u.shape != h.shape or u.dtype != h.dtype or u.data.device != h.data.device):
         raise ValueError("gate and up must be of one shape, type and device")
-    dy2 = _matrix(dy.detach())
+    dy2 = _matrix(dy)
     rows, cols = dy2.shape
-    kept = [k for k in (h, u) if k is not None]
+    kept = (h,) if u is None else (h, u)
     for k in kept:
         if tuple(k.data.shape) != (rows, cols):
             raise ValueError("the saved payload does not have its tensor's shape")
-        _plain_scale(k.scale, _scale_shape(rows, cols, "row"), k.data, "scale")
-    if not all(_plain_cuda(t) for k in kept for t in (k.data, k.scale)) or not _plain_cuda(dy2):
+        _check_scale(k.scale, _scale_shape(rows, cols, "row"), k.data, "scale")
+    if not _native(dy2, *(t for k in kept for t in (k.data, k.scale))):
         d, x = dy.detach().float(), h.restore(torch.float32)
         p = 1 / (1 + torch.exp(-x))
         slope, s = p * (1 + x * (1 - p)), x * p
         v = torch.ones_like(x) if u is None else u.restore(torch.float32)
         return (d * v * slope).to(dy.dtype), None if u is None else (d * s).to(dy.dtype), (s * v).to(dy.dtype) if act else None
-    dy2 = _rows(dy2)
-    outs = [torch.empty(rows, cols, device=dy.device, dtype=dy.dtype) if want else None for want in (True, u is not None, act)]
-    if dy2.numel():
-        ins, pitch = [], _cdiv(cols, 16) * 16
+    dy2, ld = _rows(dy2)
+    new = lambda want: torch.empty(dy.shape, device=dy.device, dtype=dy.dtype) if want else None      # noqa: E731
+    dh, du, y = new(True), new(u is not None), new(act)
+    if dh.numel():
+        pitch, ins, live = _up16(cols), [], []
         for k in kept:
-            data, p = _payload(k.data, "the saved payload")
+            data, p = _payload(k.data, "the saved payload", vectors=True)
             if p != pitch:      # a copy of what was kept may come back with rows further apart
                 data = _new_payload(rows, cols, data.device).copy_(data)
-            ins.append((data, k.scale))
-        ptrs = [v for d, s in ins for v in (d.data_ptr(), s.data_ptr(), s.stride(0), s.stride(1))] + ([None, None, 0, 0] if u is None else [])
-        _on_device(dy2, N.lib().mt_fp8_act_backward, DTYPES[dy.dtype], pitch, *ptrs, dy2.data_ptr(), _row_stride(dy2), rows, cols,
-                   *(None if t is None else t.data_ptr() for t in outs))
-    return tuple(None if t is None else t.view(dy.shape) for t in outs)
+            live.append(data)
+            ins += [data.data_ptr(), k.scale.data_ptr(), *k.scale.stride()]
+        if u is None:
+            ins += [0, 0, 0, 0]
+        _call(ACT_BACKWARD, dh.get_device(), DTYPES[dy.dtype], pitch, *ins, dy2.data_ptr(), ld, rows, cols, dh.data_ptr(),
+              du.data_ptr() if u is not None else 0, y.data_ptr() if act else 0)
+    return dh, du, y
 
 
 def silu8_forward(h: torch.Tensor) -> Tuple[torch.Tensor, Saved8]:

@@ -16,69 +16,115 @@ The reference has no fp8 path; it is on its roadmap (README.md:58-60).
 """
 from __future__ import annotations
 
+import struct
 from typing import List, Optional, Sequence, Tuple
 
 import torch
 
 from .. import _native as N
 from .mxfp8 import _QUANT_DT as DTYPES
-from .mxfp8 import _on_device, _plain_cuda
+from .mxfp8 import _plain_cuda
 
 BLOCK = 128
 BLOCKS = {"row": (1, BLOCK), "col": (BLOCK, 1), "tile": (BLOCK, BLOCK)}
 Quantized = Tuple[torch.Tensor, torch.Tensor]
+QUANTIZE, DEQUANTIZE, ACT_FORWARD, ACT_BACKWARD, GEMM, LINEAR_FORWARD, LINEAR_BACKWARD = range(7)
+_PACK = [struct.Struct(f"{n}q").pack for n in range(24)]
+_U8 = (torch.uint8, torch.float8_e4m3fn)
+_TYPES = (torch.Tensor, torch.nn.Parameter)
+_packed = None
+
+
+def _call(op: int, device: int, *args: int) -> None:
+    """Operation ``op`` (``mt_fp8_packed``) on the current stream of ``device``, with that device current."""
+    global _packed
+    if _packed is None:
+        _packed = N.lib().mt_fp8_packed
+    if device == torch._C._cuda_getDevice():
+        rc = _packed(N.raw_stream(device), op, _PACK[len(args)](*args))
+    else:
+        with torch.cuda.device(device):
+            rc = _packed(N.raw_stream(device), op, _PACK[len(args)](*args))
+    if rc < 0:
+        raise RuntimeError(f"mt_fp8 operation {op}: {N.last_error()}")
+
+
+def _recording() -> bool:
+    """Somebody records or replaces the operations on tensors: a kernel launched from here would be missing from the record."""
+    return (torch._C._get_tracing_state() is not None or torch.compiler.is_compiling()
+            or torch._C._len_torch_dispatch_stack() != 0)
+
+
+def _address(t: torch.Tensor) -> int:
+    """Where ``t`` is on a GPU, or 0: it is elsewhere, has no elements, or does not stand for its own memory (what vmap,
+    functionalisation and lazy zeros make has no address or none to be asked for)."""
+    if type(t) not in _TYPES or not t.is_cuda or t.is_neg():
+        return 0
+    try:
+        return t.data_ptr()
+    except RuntimeError:
+        return 0
+
+
+def _native(*ts: torch.Tensor) -> bool:
+    """Whether kernels may be pointed at all of these; tensors without elements count."""
+    return not _recording() and all(_address(t) or _plain_cuda(t) for t in ts)
 
 
 def _cdiv(a: int, b: int) -> int:
     return -(-a // b)
 
 
+def _up16(n: int) -> int:
+    return (n + 15) & ~15
+
+
 def _scale_shape(rows: int, cols: int, block: str) -> Tuple[int, int]:
     br, bc = BLOCKS[block]
-    return _cdiv(rows, br), _cdiv(cols, bc)
+    return -(-rows // br), -(-cols // bc)
 
 
 def _new_payload(rows: int, cols: int, device) -> torch.Tensor:
     """Rows a multiple of 16 bytes apart, as the kernels (and TMA) want them; the padding is not part of the result."""
-    pitch = _cdiv(cols, 16) * 16
-    buf = torch.empty(rows, pitch, device=device, dtype=torch.uint8)
+    pitch = _up16(cols)
+    buf = torch.empty((rows, pitch), device=device, dtype=torch.uint8)
     return buf if pitch == cols else buf[:, :cols]
 
 
 def _new_scale(rows: int, cols: int, block: str, device) -> torch.Tensor:
     r, c = _scale_shape(rows, cols, block)
-    if block == "row":   # neighbouring rows next to one another: what a warp of the product reads at once
-        return torch.empty(c, r, device=device, dtype=torch.float32).t()
-    return torch.empty(r, c, device=device, dtype=torch.float32)
+    # row blocks: neighbouring rows next to one another, what a warp of the product reads at once
+    return torch.empty_strided((r, c), (1, r) if block == "row" else (c, 1), device=device, dtype=torch.float32)
 
 
-def _row_stride(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else 0
+def _rows(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
+    """``t`` (2-D) with adjacent columns, and the elements between its rows."""
+    (rows, cols), (ld, inner) = t.shape, t.stride()
+    if cols > 1 and inner != 1:
+        return t.contiguous(), cols
+    return t, ld if rows > 1 else 0
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """``t`` (2-D) with adjacent columns."""
-    return t if t.shape[1] <= 1 or t.stride(1) == 1 else t.contiguous()
-
-
-def _payload(t: torch.Tensor, name: str) -> Tuple[torch.Tensor, int]:
-    """A payload as the kernels take it, and the bytes between its rows: copied where its rows are not on 16-byte boundaries."""
-    if t.dtype not in (torch.uint8, torch.float8_e4m3fn) or t.dim() != 2:
+def _payload(t: torch.Tensor, name: str, vectors: bool = False) -> Tuple[torch.Tensor, int]:
+    """A payload as the kernels take it, and the bytes between its rows: copied where its rows are not on 16-byte boundaries,
+    or (``vectors``: the kernel reads whole ones) where the last row's padding is not there to be read."""
+    if t.dtype not in _U8 or t.dim() != 2:
         raise ValueError(f"{name} must be a 2-D uint8 or float8_e4m3fn tensor")
-    rows, cols = t.shape
-    t = t.view(torch.uint8)
-    if cols <= 1 or t.stride(1) == 1:
-        pitch = t.stride(0) if rows > 1 else _cdiv(cols, 16) * 16
-        end = t.storage_offset() + max(rows - 1, 0) * pitch + _cdiv(cols, 16) * 16      # the last row is read in whole vectors too
-        if t.data_ptr() % 16 == 0 and pitch % 16 == 0 and pitch >= cols and end <= t.untyped_storage().nbytes():
+    (rows, cols), (pitch, inner) = t.shape, t.stride()
+    if rows <= 1:
+        pitch = _up16(cols)
+    if (cols <= 1 or inner == 1) and pitch % 16 == 0 and pitch >= cols and t.data_ptr() % 16 == 0:
+        if not vectors or cols % 16 == 0:
+            return t, pitch
+        if t.storage_offset() + (rows - 1) * pitch + _up16(cols) <= t.untyped_storage().nbytes():
             return t, pitch
     buf = _new_payload(rows, cols, t.device)
-    buf.copy_(t)
-    return buf, _cdiv(cols, 16) * 16
+    buf.copy_(t.view(torch.uint8))
+    return buf, _up16(cols)
 
 
-def _plain_scale(s: torch.Tensor, shape: Tuple[int, int], like: torch.Tensor, name: str) -> torch.Tensor:
-    if s.dtype != torch.float32 or tuple(s.shape) != shape or s.device != like.device:
+def _check_scale(s: torch.Tensor, shape: Tuple[int, int], like: torch.Tensor, name: str) -> torch.Tensor:
+    if s.dtype != torch.float32 or s.shape != shape or s.device != like.device:
         raise ValueError(f"{name} must be a float32 tensor of shape {shape} on {like.device}")
     return s
 
@@ -102,16 +148,17 @@ def quantize_fp8_many(x: torch.Tensor, blocks: Sequence[str]) -> List[Quantized]
     _check_float(x, "x")
     if not blocks or len(set(blocks)) != len(blocks) or any(b not in BLOCKS for b in blocks):
         raise ValueError(f"blocks must be different ones of {sorted(BLOCKS)}")
-    if not _plain_cuda(x):
+    if not _native(x):
         return [_torch_quantize(x, b) for b in blocks]
     rows, cols = x.shape
     out = {b: (_new_payload(rows, cols, x.device), _new_scale(rows, cols, b, x.device)) for b in blocks}
     if x.numel():
-        x = _rows(x)
-        ptrs = []
-        for b in ("row", "col", "tile"):
-            ptrs += [out[b][0].data_ptr(), out[b][1].data_ptr()] if b in out else [None, None]
-        _on_device(x, N.lib().mt_fp8_quantize, DTYPES[x.dtype], x.data_ptr(), _row_stride(x), rows, cols, _cdiv(cols, 16) * 16, *ptrs)
+        x, ld = _rows(x)
+        ptrs = [0] * 6
+        for b, (data, scale) in out.items():
+            at = 0 if b == "row" else 2 if b == "col" else 4
+            ptrs[at], ptrs[at + 1] = data.data_ptr(), scale.data_ptr()
+        _call(QUANTIZE, x.get_device(), DTYPES[x.dtype], x.data_ptr(), ld, rows, cols, _up16(cols), *ptrs)
     return [out[b] for b in blocks]
 
 
@@ -146,16 +193,16 @@ def dequantize_fp8(data: torch.Tensor, scale: torch.Tensor, block: str = "row", 
     if data.dtype not in (torch.uint8, torch.float8_e4m3fn) or data.dim() != 2:
         raise ValueError("data must be a 2-D uint8 or float8_e4m3fn tensor")
     rows, cols = data.shape
-    _plain_scale(scale, _scale_shape(rows, cols, block), data, "scale")
-    if not (_plain_cuda(data) and _plain_cuda(scale)):
+    _check_scale(scale, _scale_shape(rows, cols, block), data, "scale")
+    if not _native(data, scale):
         top = torch.finfo(dtype).max
         return (data.view(torch.float8_e4m3fn).float() * _spread(scale, rows, cols, block)).clamp(-top, top).to(dtype)
-    out = torch.empty(rows, cols, device=data.device, dtype=dtype)
+    out = torch.empty((rows, cols), device=data.device, dtype=dtype)
     if out.numel():
-        data, pitch = _payload(data, "data")
+        data, pitch = _payload(data, "data", vectors=True)
         br, bc = BLOCKS[block]
-        _on_device(data, N.lib().mt_fp8_dequantize, DTYPES[dtype], data.data_ptr(), pitch, scale.data_ptr(), scale.stride(0),
-                   scale.stride(1), rows, cols, br, bc, out.data_ptr(), cols)
+        _call(DEQUANTIZE, out.get_device(), DTYPES[dtype], data.data_ptr(), pitch, scale.data_ptr(), *scale.stride(), rows, cols, br, bc,
+              out.data_ptr(), cols)
     return out
 
 
@@ -171,64 +218,116 @@ def gemm_fp8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: t
     Sums are fp32 with one rounding to ``dtype`` (fp32, fp16 or bf16; that of ``out`` where it is given) at the end."""
     if ta and not tb:
         raise ValueError("gemm_fp8: ta goes with tb")
-    for t, name in ((a, "a"), (a_scale, "a_scale"), (b, "b"), (b_scale, "b_scale")):
-        if not _plain_cuda(t):
-            raise ValueError(f"{name} must be a plain CUDA tensor")
-        if t.device != a.device:
-            raise ValueError("operands must be on one device")
+    if not _native(a, a_scale, b, b_scale):
+        raise ValueError("operands must be plain CUDA tensors, and nobody recording")
+    device = a.device
     a, lda = _payload(a, "a")
     b, ldb = _payload(b, "b")
-    M, K = (a.shape[1], a.shape[0]) if ta else a.shape
-    Nn, K2 = (b.shape[1], b.shape[0]) if tb else b.shape
+    if b.device != device:
+        raise ValueError("operands must be on one device")
+    sa, sb = a.shape, b.shape
+    M, K = (sa[1], sa[0]) if ta else sa
+    Nn, K2 = (sb[1], sb[0]) if tb else sb
     if K != K2:
         raise ValueError("inner dimensions differ")
-    _plain_scale(a_scale, _scale_shape(*a.shape, "col" if ta else "row"), a, "a_scale")
-    _plain_scale(b_scale, _scale_shape(*b.shape, "tile"), b, "b_scale")
+    kb = -(-K // BLOCK)
+    _check_scale(a_scale, (kb, M) if ta else (M, kb), a, "a_scale")
+    _check_scale(b_scale, _scale_shape(*sb, "tile"), b, "b_scale")
     if out is None:
         if dtype not in DTYPES:
             raise ValueError("dtype must be float32, float16 or bfloat16")
-        out = torch.empty(M, Nn, device=a.device, dtype=dtype)
-    elif (tuple(out.shape) != (M, Nn) or out.dtype not in DTYPES or out.device != a.device or not _plain_cuda(out)
-          or (Nn > 1 and out.stride(1) != 1) or (M > 1 and out.stride(0) < Nn)):
-        raise ValueError("out must be a float32, float16 or bfloat16 CUDA tensor [M, N] with adjacent columns")
+        out, ldc = torch.empty((M, Nn), device=device, dtype=dtype), Nn
+    else:
+        ldc = out.stride(0) if out.dim() == 2 and M > 1 else Nn
+        if (tuple(out.shape) != (M, Nn) or out.dtype not in DTYPES or out.device != device or not _native(out)
+                or (Nn > 1 and out.stride(1) != 1) or ldc < Nn):
+            raise ValueError("out must be a float32, float16 or bfloat16 CUDA tensor [M, N] with adjacent columns")
     if not out.numel():
         return out
     if K == 0:
         return out.zero_()
-    sa_m, sa_k = (a_scale.stride(1), a_scale.stride(0)) if ta else a_scale.stride()
-    sb_n, sb_k = (b_scale.stride(1), b_scale.stride(0)) if tb else b_scale.stride()
-    _on_device(a, N.lib().mt_gemm_fp8, a.data_ptr(), lda, a_scale.data_ptr(), sa_m, sa_k, b.data_ptr(), ldb, b_scale.data_ptr(),
-               sb_n, sb_k, out.data_ptr(), out.stride(0) if M > 1 else Nn, DTYPES[out.dtype], M, Nn, K, int(ta), int(tb), nctas)
+    sa_r, sa_c = a_scale.stride()
+    sb_r, sb_c = b_scale.stride()
+    _call(GEMM, out.get_device(), a.data_ptr(), lda, a_scale.data_ptr(), *((sa_c, sa_r) if ta else (sa_r, sa_c)), b.data_ptr(), ldb,
+          b_scale.data_ptr(), *((sb_c, sb_r) if tb else (sb_r, sb_c)), out.data_ptr(), ldc, DTYPES[out.dtype], M, Nn, K, int(ta), int(tb),
+          nctas)
     return out
+
+
+# ---- the linear layer ----------------------------------------------------------------------------------------------
+def _areas(*sizes: int) -> Tuple[List[int], int]:
+    """Offsets of areas of these sizes in one buffer (allocating each by itself is most of a small layer's time), and its size."""
+    offs, at = [], 0
+    for n in sizes:
+        offs.append(at)
+        at += (n + 255) & ~255
+    return offs, at
+
+
+def _sizes(rows: int, cols: int, block: str) -> Tuple[int, int]:
+    r, c = _scale_shape(rows, cols, block)
+    return rows * _up16(cols), 4 * r * c
 
 
 class _LinearFp8(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, w_data, w_scale, keep):
-        x2 = x.reshape(-1, x.shape[-1])
         # keep: the weight has a gradient, which contracts over the tokens; what is kept of x for it are tiles, in 8 bits
-        q = quantize_fp8_many(x2, ("row", "tile") if keep else ("row",))
-        if w_data is None:
-            w_data, w_scale = quantize_fp8(w, "tile")
-        y = gemm_fp8(*q[0], w_data, w_scale, dtype=x.dtype)
-        ctx.save_for_backward(*(q[1] if keep else (None, None)), w_data, w_scale)
-        ctx.dtypes = x.dtype, w.dtype
-        return y.view(*x.shape[:-1], w.shape[0])
+        (n, k), dev = w.shape, x.device
+        x2, ldx = _rows(x.reshape(-1, k))
+        t = x2.shape[0]
+        own = w_data is None
+        offs, size = _areas(*(_sizes(t, k, "tile") if keep else (0, 0)), *(_sizes(n, k, "tile") if own else (0, 0)))
+        kept = torch.empty(size, device=dev, dtype=torch.uint8) if size else None
+        base = kept.data_ptr() if size else 0
+        ctx.sizes = t, n, k, offs, size, x.dtype, w.dtype
+        ctx.save_for_backward(kept, w_data, w_scale)
+        y = torch.empty((*x.shape[:-1], n), device=dev, dtype=x.dtype)
+        if own:
+            w2, ldw = _rows(w.detach())
+            wq = w2.data_ptr(), ldw, base + offs[2], _up16(k), base + offs[3], -(-k // BLOCK), 1
+        else:
+            w2, pitch = _payload(w_data, "w_fp8")
+            wq = 0, 0, w2.data_ptr(), pitch, w_scale.data_ptr(), *w_scale.stride()
+        if t:
+            (data_at, scale_at), room = _areas(*_sizes(t, k, "row"))
+            tmp = torch.empty(room, device=dev, dtype=torch.uint8)
+            at = tmp.data_ptr()
+            _call(LINEAR_FORWARD, y.get_device(), DTYPES[x.dtype], x2.data_ptr(), ldx, t, k, DTYPES[w.dtype], wq[0], wq[1], n,
+                  at + data_at, at + scale_at, *((base + offs[0], base + offs[1]) if keep else (0, 0)), *wq[2:], y.data_ptr())
+        elif own:
+            _call(QUANTIZE, y.get_device(), DTYPES[w.dtype], wq[0], wq[1], n, k, wq[3], 0, 0, 0, 0, wq[2], wq[4])
+        return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        xt, xt_scale, w_data, w_scale = ctx.saved_tensors
+        kept, w_data, w_scale = ctx.saved_tensors
+        t, n, k, offs, size, x_dtype, w_dtype = ctx.sizes
         want_x, want_w = ctx.needs_input_grad[:2]
-        blocks = [b for b, want in (("row", want_x), ("col", want_w)) if want]
-        if not blocks:
-            return None, None, None, None, None
-        q = dict(zip(blocks, quantize_fp8_many(dy.reshape(-1, dy.shape[-1]), blocks)))
-        dx = dw = None
-        if want_x:
-            dx = gemm_fp8(*q["row"], w_data, w_scale, tb=True, dtype=ctx.dtypes[0]).view(*dy.shape[:-1], w_data.shape[1])
-        if want_w:
-            dw = gemm_fp8(*q["col"], xt, xt_scale, ta=True, tb=True, dtype=ctx.dtypes[1])
+        base = 0
+        if size:   # what a saved-tensor hook made of it
+            kept = kept.contiguous()
+            if kept.data_ptr() % 16:
+                kept = kept.clone()
+            base = kept.data_ptr()
+        if w_data is None:
+            w2, wq = None, (base + offs[2], _up16(k), base + offs[3], -(-k // BLOCK), 1)
+        else:
+            w2, pitch = _payload(w_data, "w_fp8")
+            wq = w2.data_ptr(), pitch, w_scale.data_ptr(), *w_scale.stride()
+        dx = torch.empty((*dy.shape[:-1], k), device=dy.device, dtype=x_dtype) if want_x else None
+        dw = torch.empty((n, k), device=dy.device, dtype=w_dtype) if want_w else None
+        if t and (want_x or want_w):
+            dy2, ld = _rows(dy.reshape(-1, n))
+            (rd, rs, cd, cs), room = _areas(*(_sizes(t, n, "row") if want_x else (0, 0)), *(_sizes(t, n, "col") if want_w else (0, 0)))
+            tmp = torch.empty(room, device=dy.device, dtype=torch.uint8)
+            at = tmp.data_ptr()
+            _call(LINEAR_BACKWARD, dy.get_device(), DTYPES[x_dtype], dy2.data_ptr(), ld, t, n, k, at + rd, at + rs, *wq,
+                  dx.data_ptr() if want_x else 0, at + cd, at + cs, base + offs[0], base + offs[1], dw.data_ptr() if want_w else 0,
+                  DTYPES[w_dtype])
+        elif want_w:
+            dw.zero_()
         return dx, dw, None, None, None
 
 
@@ -247,7 +346,11 @@ def linear_fp8(x: torch.Tensor, w: torch.Tensor, w_fp8: Optional[Quantized] = No
         raise ValueError("x and w must be on one CUDA device")
     if 0 in w.shape:
         raise ValueError("w has no elements")
+    if not _native(x, w):
+        raise ValueError("x and w must be plain CUDA tensors, and nobody recording")
     data, scale = w_fp8 if w_fp8 is not None else (None, None)
-    if data is not None and tuple(data.shape) != tuple(w.shape):
-        raise ValueError("w_fp8 does not belong to w")
+    if data is not None:
+        if data.shape != w.shape or data.dtype not in _U8 or not _native(data, scale) or data.device != w.device:
+            raise ValueError("w_fp8 does not belong to w")
+        _check_scale(scale, _scale_shape(*w.shape, "tile"), data, "the scales of w_fp8")
     return _LinearFp8.apply(x, w, data, scale, torch.is_grad_enabled() and w.requires_grad)
