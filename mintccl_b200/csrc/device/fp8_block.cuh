@@ -5,6 +5,8 @@
 #include <cuda_fp8.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "prims.cuh"
 #include "reduce_ops.cuh"
 
@@ -22,12 +24,9 @@ __device__ __forceinline__ float fp8_scale(uint32_t e) { return __uint_as_float(
 __device__ __forceinline__ float fp8_inverse(uint32_t e) { return __uint_as_float((254u - e) << 23); }   // e <= 247
 
 __device__ __forceinline__ uint32_t abs_bits(float f) { return __float_as_uint(f) & 0x7fffffffu; }
-__device__ __forceinline__ uint32_t finite_bits(float f) {
-  const uint32_t b = abs_bits(f);
-  return b < kInfBits ? b : 0u;
-}
-// 16 values (quotients by the scale) as e4m3.  `special`: some may not be finite.
-__device__ __forceinline__ uint4 e4m3_16(const float* f, float inv, bool special) {
+// 16 values times inv as e4m3.  SPECIAL: some may not be finite.
+template <bool SPECIAL>
+__device__ __forceinline__ uint4 e4m3_16(const float* f, float inv) {
   uint32_t w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -35,7 +34,7 @@ __device__ __forceinline__ uint4 e4m3_16(const float* f, float inv, bool special
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       v[j] = f[4 * i + j] * inv;
-      if (special && abs_bits(f[4 * i + j]) >= kInfBits) v[j] = __uint_as_float(0x7fc00000u);
+      if (SPECIAL && abs_bits(f[4 * i + j]) >= kInfBits) v[j] = __uint_as_float(0x7fc00000u);
     }
     w[i] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(v[0], v[1]), __NV_SATFINITE, __NV_E4M3) |
            ((uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(v[2], v[3]), __NV_SATFINITE, __NV_E4M3) << 16);
@@ -96,6 +95,13 @@ struct Span16 {
       for (int i = 0; i < kWords; ++i) v[i] = i < n ? __ldg(e + i) : 0u;
     }
   }
+  __device__ __forceinline__ void clear(int n) {   // elements from the n-th on
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+      if constexpr (sizeof(E) == 2) v[i] = 2 * i + 1 < n ? v[i] : 2 * i < n ? v[i] & 0xffffu : 0u;
+      else v[i] = i < n ? v[i] : 0u;
+    }
+  }
   __device__ __forceinline__ void get(float* f) const {
 #pragma unroll
     for (int i = 0; i < kWords / 2; ++i) T::unpack((uint64_t)v[2 * i] | ((uint64_t)v[2 * i + 1] << 32), f + i * T::kPer64);
@@ -133,6 +139,114 @@ struct Span16 {
     }
   }
 };
+// The same for a whole warp, whose lanes have the spans of four blocks of 128, eight lanes each.  By elements the blocks go
+// through shared memory (kStage bytes a warp), neighbouring elements on neighbouring lanes: a lane that reads or writes its
+// own 16 elements one by one touches as many sectors with every instruction as the warp has lanes (3000 x 4095 in bf16,
+// decoding: 67 us that way, 17 encoding).
+template <class T, int VEC>
+struct WarpSpans {
+  using E = typename T::elem;
+  static constexpr int kPitch = 128 * (int)sizeof(E) + 16, kStage = VEC ? 16 : 4 * kPitch;
+  // p: the lane's span, n: elements of the lane's that exist
+  static __device__ __forceinline__ void load(Span16<T, VEC>& v, const uint8_t* p, int n, uint8_t* stage) {
+    if constexpr (VEC > 0) {
+      v.load(p, n);
+    } else {
+      const int lane = threadIdx.x & 31;
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const E* from = (const E*)(uintptr_t)__shfl_sync(0xffffffffu, (unsigned long long)(uintptr_t)p, 8 * b);
+        const int have = __reduce_add_sync(0xffffffffu, (lane >> 3) == b ? n : 0);
+        E e[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (i * 32 + lane < have) e[i] = from[i * 32 + lane];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (i * 32 + lane < have) ((E*)(stage + b * kPitch))[i * 32 + lane] = e[i];
+      }
+      __syncwarp();
+      const uint4* mine = (const uint4*)(stage + (lane >> 3) * kPitch + (lane & 7) * 16 * sizeof(E));
+#pragma unroll
+      for (int i = 0; i < Span16<T, VEC>::kWords / 4; ++i) {
+        const uint4 t = mine[i];
+        v.v[4 * i] = t.x;
+        v.v[4 * i + 1] = t.y;
+        v.v[4 * i + 2] = t.z;
+        v.v[4 * i + 3] = t.w;
+      }
+      v.clear(n);
+      __syncwarp();
+    }
+  }
+  static __device__ __forceinline__ void store(const Span16<T, VEC>& v, uint8_t* p, int n, uint8_t* stage) {
+    if constexpr (VEC > 0) {
+      v.store(p, n);
+    } else {
+      const int lane = threadIdx.x & 31;
+      uint4* mine = (uint4*)(stage + (lane >> 3) * kPitch + (lane & 7) * 16 * sizeof(E));
+#pragma unroll
+      for (int i = 0; i < Span16<T, VEC>::kWords / 4; ++i) mine[i] = make_uint4(v.v[4 * i], v.v[4 * i + 1], v.v[4 * i + 2], v.v[4 * i + 3]);
+      __syncwarp();
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        E* to = (E*)(uintptr_t)__shfl_sync(0xffffffffu, (unsigned long long)(uintptr_t)p, 8 * b);
+        const int have = __reduce_add_sync(0xffffffffu, (lane >> 3) == b ? n : 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (i * 32 + lane < have) to[i * 32 + lane] = ((const E*)(stage + b * kPitch))[i * 32 + lane];
+      }
+      __syncwarp();
+    }
+  }
+};
+
+// Magnitudes as integers, which order as the values do, NaN above everything: 16-bit types two to a word.
+template <class T>
+struct Mags {
+  static constexpr bool kHalf = sizeof(typename T::elem) == 2;
+  static constexpr int kWords = kHalf ? 8 : 16;
+  uint32_t m[kWords];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) m[i] = 0;
+  }
+  static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return kHalf ? __vmaxu2(a, b) : max(a, b); }
+  static __device__ __forceinline__ uint32_t mag(uint32_t v) { return v & (kHalf ? 0x7fff7fffu : 0x7fffffffu); }
+  // with what is not finite counted as nothing
+  static __device__ __forceinline__ uint32_t finite(uint32_t v) {
+    const uint32_t a = mag(v);
+    if constexpr (!kHalf) {
+      return a < kInfBits ? a : 0u;
+    } else {
+      const uint32_t inf = std::is_same<T, F16>::value ? 0x7c00u : 0x7f80u;
+      return ((a & 0xffffu) < inf ? a & 0xffffu : 0u) | ((a >> 16) < inf ? a & 0xffff0000u : 0u);
+    }
+  }
+  template <bool FINITE>
+  __device__ __forceinline__ void fold(const uint32_t* v) {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) m[i] = larger(m[i], FINITE ? finite(v[i]) : mag(v[i]));
+  }
+  // fp32 bits of one magnitude
+  static __device__ __forceinline__ uint32_t bits(uint32_t h) {
+    if constexpr (!kHalf) return h;
+    else if constexpr (std::is_same<T, BF16>::value) return h << 16;
+    else return __float_as_uint(__half2float(__ushort_as_half((unsigned short)h)));
+  }
+  __device__ __forceinline__ uint32_t of(int column) const {   // raw, before bits()
+    if constexpr (!kHalf) return m[column];
+    else return (column & 1) ? m[column >> 1] >> 16 : m[column >> 1] & 0xffffu;
+  }
+  __device__ __forceinline__ uint32_t top() const {            // fp32 bits of the largest
+    uint32_t t = m[0];
+#pragma unroll
+    for (int i = 1; i < kWords; ++i) t = larger(t, m[i]);
+    if constexpr (kHalf) t = max(t & 0xffffu, t >> 16);
+    return bits(t);
+  }
+};
+
 // Largest finite value of a type, for restored values that rounding took past it.
 template <class T>
 struct MaxOf;
@@ -150,50 +264,73 @@ __device__ __forceinline__ float clamp_nan(float v, float m) {
 }
 
 // Where a thread of the row-block kernels works: eight lanes share a block of 128, 16 elements each, and a CTA of 256
-// threads has 32 blocks per step: 32 rows where there are that many (their scales are neighbours in memory), else 32
-// blocks that follow one another along the rows.
+// threads has 32 blocks an item: of 32 rows where there are that many (their scales are neighbours in memory), else 32
+// blocks of one row.  Items are counted in 32 bits: a 64-bit division costs as much as a block.
 struct RowSpan {
-  int64_t row, kb;
+  int64_t row;
+  uint32_t kb;
   bool live;
 };
-__device__ __forceinline__ RowSpan row_span(int64_t item, int g, int64_t rows, int64_t nkb, bool by_rows) {
+__host__ __device__ __forceinline__ int64_t row_items(int64_t rows, int64_t nkb) {
+  return rows >= 32 ? (rows + 31) / 32 * nkb : rows * ((nkb + 31) / 32);
+}
+__device__ __forceinline__ RowSpan row_span(uint32_t item, int g, int64_t rows, uint32_t nkb) {
   RowSpan r;
-  if (by_rows) {
-    const int64_t rt = item / nkb;
+  if (rows >= 32) {
+    const uint32_t rt = item / nkb;
     r.kb = item - rt * nkb;
-    r.row = rt * 32 + g;
+    r.row = (int64_t)rt * 32 + g;
     r.live = r.row < rows;
   } else {
-    const int64_t id = item * 32 + g;
-    r.row = id / nkb;
-    r.kb = id - r.row * nkb;
-    r.live = r.row < rows;
+    const uint32_t chunks = (nkb + 31) / 32, row = item / chunks;
+    r.row = row;
+    r.kb = (item - row * chunks) * 32 + g;
+    r.live = r.row < rows && r.kb < nkb;
   }
   return r;
 }
-// One step of a CTA is an item; this many there are.
-__host__ __device__ __forceinline__ int64_t row_items(int64_t rows, int64_t nkb, bool by_rows) {
-  return by_rows ? (rows + 31) / 32 * nkb : (rows * nkb + 31) / 32;
-}
 
-// Encodes the 16 values of this lane as part of its row block.  All lanes of the warp take part.
-__device__ __forceinline__ uint4 encode_row16(const float* f, uint32_t* exp_out) {
-  uint32_t m = 0;
+// fp32 bits of the largest finite magnitudes of the row blocks that this lane's spans are parts of, all lanes of the warp
+// together; true if something in them was not finite.
+template <class T, int VEC, int U>
+__device__ __forceinline__ bool row_tops(const Span16<T, VEC>* v, uint32_t* top) {
+  auto reduce = [&] {
 #pragma unroll
-  for (int i = 0; i < 16; ++i) m = max(m, abs_bits(f[i]));
+    for (int d = 1; d < 8; d <<= 1)
 #pragma unroll
-  for (int d = 1; d < 8; d <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
-  const bool special = __any_sync(0xffffffffu, m >= kInfBits);
-  if (special) {
-    m = 0;
+      for (int u = 0; u < U; ++u) top[u] = max(top[u], __shfl_xor_sync(0xffffffffu, top[u], d));
+  };
+  Mags<T> m;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) m = max(m, finite_bits(f[i]));
-#pragma unroll
-    for (int d = 1; d < 8; d <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
+  for (int u = 0; u < U; ++u) {
+    m.clear();
+    m.template fold<false>(v[u].v);
+    top[u] = m.top();
   }
-  const uint32_t e = fp8_scale_exp(m);
-  *exp_out = e;
-  return e4m3_16(f, fp8_inverse(e), special);
+  reduce();
+  uint32_t all = top[0];
+#pragma unroll
+  for (int u = 1; u < U; ++u) all = max(all, top[u]);
+  const bool special = __any_sync(0xffffffffu, all >= kInfBits);
+  if (special) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      m.clear();
+      m.template fold<true>(v[u].v);
+      top[u] = m.top();
+    }
+    reduce();
+  }
+  return special;
+}
+// Encodes the 16 values of this lane as part of its row block.  All lanes of the warp take part.
+template <class T, int VEC>
+__device__ __forceinline__ uint4 encode_row16(const Span16<T, VEC>& v, const float* f, uint32_t* exp_out) {
+  uint32_t top;
+  const bool special = row_tops<T, VEC, 1>(&v, &top);
+  *exp_out = fp8_scale_exp(top);
+  const float inv = fp8_inverse(*exp_out);
+  return special ? e4m3_16<true>(f, inv) : e4m3_16<false>(f, inv);
 }
 
 }  // namespace mt

@@ -49,62 +49,70 @@ __device__ __forceinline__ float silu_of(float x) {
 }
 
 template <class T, int VEC, bool GATED>
-__global__ void __launch_bounds__(kThreads) fp8_act_fwd_kernel(Fp8ActArgs a, int64_t nkb, bool by_rows) {
+__global__ void __launch_bounds__(kThreads) fp8_act_fwd_kernel(Fp8ActArgs a, uint32_t nkb) {
   using E = typename T::elem;
+  using W = WarpSpans<T, VEC>;
   constexpr int kE = (int)sizeof(E);
   constexpr bool kExact = kE == 4;
+  __shared__ __align__(16) uint8_t stages[8][W::kStage];
+  uint8_t* stage = stages[threadIdx.x >> 5];
   const int g = threadIdx.x >> 3, l = threadIdx.x & 7;
-  const RowSpan at = row_span(blockIdx.x, g, a.rows, nkb, by_rows);
-  const int64_t c0 = at.kb * 128 + l * 16;
+  const RowSpan at = row_span(blockIdx.x, g, a.rows, nkb);
+  const int64_t c0 = (int64_t)at.kb * 128 + l * 16;
   const int n = at.live ? (int)min((int64_t)16, max((int64_t)0, a.cols - c0)) : 0;
   Span16<T, VEC> h, u;
-  h.load((const uint8_t*)a.h + (at.row * a.ldh + c0) * kE, n);
-  if (GATED) u.load((const uint8_t*)a.u + (at.row * a.ldu + c0) * kE, n);
+  W::load(h, (const uint8_t*)a.h + (at.row * a.ldh + c0) * kE, n, stage);
+  if (GATED) W::load(u, (const uint8_t*)a.u + (at.row * a.ldu + c0) * kE, n, stage);
   const bool put = at.live && c0 < a.ldq;
   float f[16], y[16];
   uint32_t e;
   h.get(f);
 #pragma unroll
   for (int i = 0; i < 16; ++i) y[i] = silu_of<kExact>(f[i]);
-  uint4 q = encode_row16(f, &e);
+  uint4 q = encode_row16(h, f, &e);
   if (put) *(uint4*)(a.kh.data + at.row * a.ldq + c0) = q;
   if (at.live && l == 0) a.kh.scale[at.row * a.kh.s_row + at.kb * a.kh.s_col] = fp8_scale(e);
   if (GATED) {
     u.get(f);
 #pragma unroll
     for (int i = 0; i < 16; ++i) y[i] *= f[i];
-    q = encode_row16(f, &e);
+    q = encode_row16(u, f, &e);
     if (put) *(uint4*)(a.ku.data + at.row * a.ldq + c0) = q;
     if (at.live && l == 0) a.ku.scale[at.row * a.ku.s_row + at.kb * a.ku.s_col] = fp8_scale(e);
   }
-  if (n > 0) {
-    h.set(y);
-    h.store((uint8_t*)a.y + (at.row * a.ldy + c0) * kE, n);
-  }
+  h.set(y);
+  W::store(h, (uint8_t*)a.y + (at.row * a.ldy + c0) * kE, n, stage);
 }
 
 template <class T, int VEC, bool GATED>
-__global__ void __launch_bounds__(kThreads) fp8_act_bwd_kernel(Fp8ActArgs a, int64_t nkb, bool by_rows) {
+__global__ void __launch_bounds__(kThreads) fp8_act_bwd_kernel(Fp8ActArgs a, uint32_t nkb) {
   using E = typename T::elem;
+  using W = WarpSpans<T, VEC>;
   constexpr int kE = (int)sizeof(E);
   constexpr bool kExact = kE == 4;
+  __shared__ __align__(16) uint8_t stages[8][W::kStage];
+  uint8_t* stage = stages[threadIdx.x >> 5];
   const int g = threadIdx.x >> 3, l = threadIdx.x & 7;
-  const RowSpan at = row_span(blockIdx.x, g, a.rows, nkb, by_rows);
-  const int64_t c0 = at.kb * 128 + l * 16;
-  if (!at.live || c0 >= a.cols) return;
-  const int n = (int)min((int64_t)16, a.cols - c0);
+  const RowSpan at = row_span(blockIdx.x, g, a.rows, nkb);
+  const int64_t c0 = (int64_t)at.kb * 128 + l * 16;
+  const int n = at.live ? (int)min((int64_t)16, max((int64_t)0, a.cols - c0)) : 0;
+  if (VEC > 0 && n <= 0) return;   // by elements the warp works as one
+  u128 hq = {0, 0}, uq = {0, 0};
+  float hs = 0.f, us = 0.f;
+  if (VEC > 0 || n > 0) {
+    hq = load128_stream(a.kh.data + at.row * a.ldq + c0);
+    hs = __ldg(a.kh.scale + at.row * a.kh.s_row + at.kb * a.kh.s_col);
+    if (GATED) {
+      uq = load128_stream(a.ku.data + at.row * a.ldq + c0);
+      us = __ldg(a.ku.scale + at.row * a.ku.s_row + at.kb * a.ku.s_col);
+    }
+  }
   Span16<T, VEC> d;
-  d.load((const uint8_t*)a.dy + (at.row * a.lddy + c0) * kE, n);
-  const u128 hq = load128_stream(a.kh.data + at.row * a.ldq + c0);
-  u128 uq = hq;
-  if (GATED) uq = load128_stream(a.ku.data + at.row * a.ldq + c0);
-  const float hs = __ldg(a.kh.scale + at.row * a.kh.s_row + at.kb * a.kh.s_col);
-  const float us = GATED ? __ldg(a.ku.scale + at.row * a.ku.s_row + at.kb * a.ku.s_col) : 1.f;
-  float h[16], u[16], f[16];
+  W::load(d, (const uint8_t*)a.dy + (at.row * a.lddy + c0) * kE, n, stage);
+  float h[16], u[16], f[16], act[16];
   e4m3_16_to_float(make_uint4((uint32_t)hq.x, (uint32_t)(hq.x >> 32), (uint32_t)hq.y, (uint32_t)(hq.y >> 32)), h);
   if (GATED) e4m3_16_to_float(make_uint4((uint32_t)uq.x, (uint32_t)(uq.x >> 32), (uint32_t)uq.y, (uint32_t)(uq.y >> 32)), u);
   d.get(f);
-  float act[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     const float x = clamp_nan(h[i] * hs, 3.4028234663852886e38f);
@@ -121,30 +129,29 @@ __global__ void __launch_bounds__(kThreads) fp8_act_bwd_kernel(Fp8ActArgs a, int
     }
   }
   d.set(h);
-  d.store((uint8_t*)a.dh + (at.row * a.lddh + c0) * kE, n);
+  W::store(d, (uint8_t*)a.dh + (at.row * a.lddh + c0) * kE, n, stage);
   if (GATED) {
     d.set(u);
-    d.store((uint8_t*)a.du + (at.row * a.lddu + c0) * kE, n);
+    W::store(d, (uint8_t*)a.du + (at.row * a.lddu + c0) * kE, n, stage);
   }
   if (a.y) {
     d.set(act);
-    d.store((uint8_t*)a.y + (at.row * a.ldy + c0) * kE, n);
+    W::store(d, (uint8_t*)a.y + (at.row * a.ldy + c0) * kE, n, stage);
   }
 }
 
 template <class T, int VEC>
 cudaError_t act_go(const Fp8ActArgs& a, bool forward, cudaStream_t s) {
-  const int64_t nkb = (a.cols + 127) / 128;
-  const bool by_rows = a.rows >= 32, gated = forward ? a.u != nullptr : a.ku.data != nullptr;
-  const int64_t items = row_items(a.rows, nkb, by_rows);
+  const int64_t nkb = (a.cols + 127) / 128, items = row_items(a.rows, nkb);
+  const bool gated = forward ? a.u != nullptr : a.ku.data != nullptr;
   if (items >= 0x7fffffffll) return cudaErrorInvalidValue;
-  const unsigned grid = (unsigned)items;
+  auto go = [&](auto kernel) { kernel<<<(unsigned)items, kThreads, 0, s>>>(a, (uint32_t)nkb); };
   if (forward) {
-    if (gated) fp8_act_fwd_kernel<T, VEC, true><<<grid, kThreads, 0, s>>>(a, nkb, by_rows);
-    else fp8_act_fwd_kernel<T, VEC, false><<<grid, kThreads, 0, s>>>(a, nkb, by_rows);
+    if (gated) go(fp8_act_fwd_kernel<T, VEC, true>);
+    else go(fp8_act_fwd_kernel<T, VEC, false>);
   } else {
-    if (gated) fp8_act_bwd_kernel<T, VEC, true><<<grid, kThreads, 0, s>>>(a, nkb, by_rows);
-    else fp8_act_bwd_kernel<T, VEC, false><<<grid, kThreads, 0, s>>>(a, nkb, by_rows);
+    if (gated) go(fp8_act_bwd_kernel<T, VEC, true>);
+    else go(fp8_act_bwd_kernel<T, VEC, false>);
   }
   return cudaGetLastError();
 }

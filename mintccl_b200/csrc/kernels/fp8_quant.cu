@@ -4,6 +4,8 @@
 // The reference has no fp8 path; it is on its roadmap (README.md:58-60).
 #include <cuda_runtime.h>
 
+#include <type_traits>
+
 #include "../device/fp8_block.cuh"
 #include "fp8.h"
 #include "launch.h"
@@ -15,98 +17,108 @@ constexpr int kThreads = 256;
 
 // ---- row blocks: eight lanes a block, U blocks of every lane group in flight
 template <class T, int VEC, int U>
-__global__ void __launch_bounds__(kThreads) fp8_row_kernel(Fp8QuantArgs a, int64_t nkb, int64_t items, bool by_rows) {
+__global__ void __launch_bounds__(kThreads) fp8_row_kernel(Fp8QuantArgs a, uint32_t nkb, uint32_t items) {
   constexpr int kE = (int)sizeof(typename T::elem);
+  using W = WarpSpans<T, VEC>;
+  __shared__ __align__(16) uint8_t stage[8][W::kStage];
   const int g = threadIdx.x >> 3, l = threadIdx.x & 7;
   Span16<T, VEC> in[U];
   RowSpan at[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int64_t item = (int64_t)blockIdx.x * U + u;
-    at[u] = row_span(item, g, a.rows, nkb, by_rows);
+    const uint32_t item = blockIdx.x * U + u;
+    at[u] = row_span(min(item, items - 1), g, a.rows, nkb);
     at[u].live = at[u].live && item < items;
-    const int64_t c0 = at[u].kb * 128 + l * 16;
+    const int64_t c0 = (int64_t)at[u].kb * 128 + l * 16;
     const int n = at[u].live ? (int)min((int64_t)16, max((int64_t)0, a.cols - c0)) : 0;
-    in[u].load((const uint8_t*)a.x + (at[u].row * a.ldx + c0) * kE, n);
+    W::load(in[u], (const uint8_t*)a.x + (at[u].row * a.ldx + c0) * kE, n, stage[threadIdx.x >> 5]);
   }
+  uint32_t top[U];
+  const bool special = row_tops<T, VEC, U>(in, top);
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     float f[16];
     in[u].get(f);
-    uint32_t e;
-    const uint4 q = encode_row16(f, &e);
+    const uint32_t e = fp8_scale_exp(top[u]);
+    const uint4 q = special ? e4m3_16<true>(f, fp8_inverse(e)) : e4m3_16<false>(f, fp8_inverse(e));
     if (!at[u].live) continue;
-    const int64_t c0 = at[u].kb * 128 + l * 16;
+    const int64_t c0 = (int64_t)at[u].kb * 128 + l * 16;
     if (c0 < a.ldq) *(uint4*)(a.row.data + at[u].row * a.ldq + c0) = q;   // the padding of a row is zeros
     if (l == 0) a.row.scale[at[u].row * a.row.s_row + at[u].kb * a.row.s_col] = fp8_scale(e);
   }
 }
 
 // ---- any of the three from one read: a CTA holds a tile of 128 x 128 in registers, a thread 4 rows (32 apart) of 16
-// adjacent columns
-template <class T, int VEC>
-__global__ void __launch_bounds__(kThreads) fp8_tile_kernel(Fp8QuantArgs a, int64_t nct) {
+// adjacent columns.  Largest magnitudes are taken on the bit patterns, two to a word; tiles with values that are not finite
+// look at them again.
+template <class T, int VEC, bool ROW, bool COL, bool TILE>
+__global__ void __launch_bounds__(kThreads, sizeof(typename T::elem) == 2 && !ROW ? 3 : 2) fp8_tile_kernel(Fp8QuantArgs a, uint32_t nct) {
   constexpr int kE = (int)sizeof(typename T::elem);
-  __shared__ uint32_t s_max[8][128];
+  using M = Mags<T>;
+  using W = WarpSpans<T, VEC>;
+  __shared__ __align__(16) uint8_t stage[8][W::kStage];
+  __shared__ uint32_t s_max[8][8 * M::kWords];   // column magnitudes as words, per warp
+  __shared__ __align__(16) float s_inv[128];
   __shared__ uint32_t s_tile[8];
   const int g = threadIdx.x >> 3, l = threadIdx.x & 7, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t rt = blockIdx.x / nct, ct = blockIdx.x - rt * nct;
-  const int64_t c0 = ct * 128 + l * 16;
+  const uint32_t rt = blockIdx.x / nct, ct = blockIdx.x - rt * nct;
+  const int64_t c0 = (int64_t)ct * 128 + l * 16;
   const int n = (int)min((int64_t)16, max((int64_t)0, a.cols - c0));
   Span16<T, VEC> in[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int64_t r = rt * 128 + i * 32 + g;
-    in[i].load((const uint8_t*)a.x + (r * a.ldx + c0) * kE, r < a.rows ? n : 0);
+    const int64_t r = (int64_t)rt * 128 + i * 32 + g;
+    W::load(in[i], (const uint8_t*)a.x + (r * a.ldx + c0) * kE, r < a.rows ? n : 0, stage[warp]);
   }
-  if (a.row.data) {
+  if (ROW) {
+    uint32_t top[4];
+    const bool special = row_tops<T, VEC, 4>(in, top);
+    auto put = [&](auto SPECIAL) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int64_t r = rt * 128 + i * 32 + g;
-      float f[16];
-      in[i].get(f);
-      uint32_t e;
-      const uint4 q = encode_row16(f, &e);
-      if (r < a.rows) {
-        if (c0 < a.ldq) *(uint4*)(a.row.data + r * a.ldq + c0) = q;
-        if (l == 0) a.row.scale[r * a.row.s_row + ct * a.row.s_col] = fp8_scale(e);
+      for (int i = 0; i < 4; ++i) {
+        const int64_t r = (int64_t)rt * 128 + i * 32 + g;
+        float f[16];
+        in[i].get(f);
+        const uint32_t e = fp8_scale_exp(top[i]);
+        const uint4 q = e4m3_16<decltype(SPECIAL)::value>(f, fp8_inverse(e));
+        if (r < a.rows) {
+          if (c0 < a.ldq) *(uint4*)(a.row.data + r * a.ldq + c0) = q;
+          if (l == 0) a.row.scale[r * a.row.s_row + ct * a.row.s_col] = fp8_scale(e);
+        }
       }
+    };
+    if (special) put(std::true_type());
+    else put(std::false_type());
+  }
+  if (!COL && !TILE) return;
+  M m;
+  auto reduce = [&] {   // this warp's columns and tile to shared memory
+    if (TILE) {
+      const uint32_t t = __reduce_max_sync(0xffffffffu, m.top());
+      if (lane == 0) s_tile[warp] = t;
     }
-  }
-  if (!a.col.data && !a.tile.data) return;
-  // largest finite magnitudes of the columns, then of the tile
-  uint32_t m[16];
+    if (COL) {
 #pragma unroll
-  for (int j = 0; j < 16; ++j) m[j] = 0;
-  bool special = false;
+      for (int d = 8; d < 32; d <<= 1)
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float f[16];
-    in[i].get(f);
+        for (int j = 0; j < M::kWords; ++j) m.m[j] = M::larger(m.m[j], __shfl_xor_sync(0xffffffffu, m.m[j], d));
+      if (lane < 8)
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      special |= abs_bits(f[j]) >= kInfBits;
-      m[j] = max(m[j], finite_bits(f[j]));
+        for (int j = 0; j < M::kWords; ++j) s_max[warp][l * M::kWords + j] = m.m[j];
     }
+  };
+  m.clear();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m.template fold<false>(in[i].v);
+  const bool special = __syncthreads_or(m.top() >= kInfBits);
+  if (special) {
+    m.clear();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m.template fold<true>(in[i].v);
   }
-  if (a.tile.data) {
-    uint32_t t = 0;
-#pragma unroll
-    for (int j = 0; j < 16; ++j) t = max(t, m[j]);
-    t = __reduce_max_sync(0xffffffffu, t);
-    if (lane == 0) s_tile[warp] = t;
-  }
-  if (a.col.data) {
-#pragma unroll
-    for (int d = 8; d < 32; d <<= 1)
-#pragma unroll
-      for (int j = 0; j < 16; ++j) m[j] = max(m[j], __shfl_xor_sync(0xffffffffu, m[j], d));
-    if (lane < 8)
-#pragma unroll
-      for (int j = 0; j < 16; ++j) s_max[warp][l * 16 + j] = m[j];
-  }
+  reduce();
   __syncthreads();
-  if (a.tile.data) {
+  if (TILE) {
     uint32_t t = 0;
 #pragma unroll
     for (int w = 0; w < 8; ++w) t = max(t, s_tile[w]);
@@ -114,38 +126,44 @@ __global__ void __launch_bounds__(kThreads) fp8_tile_kernel(Fp8QuantArgs a, int6
     const float inv = fp8_inverse(e);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int64_t r = rt * 128 + i * 32 + g;
+      const int64_t r = (int64_t)rt * 128 + i * 32 + g;
       float f[16];
       in[i].get(f);
-      if (r < a.rows && c0 < a.ldq) *(uint4*)(a.tile.data + r * a.ldq + c0) = e4m3_16(f, inv, special);
+      const uint4 q = special ? e4m3_16<true>(f, inv) : e4m3_16<false>(f, inv);
+      if (r < a.rows && c0 < a.ldq) *(uint4*)(a.tile.data + r * a.ldq + c0) = q;
     }
     if (threadIdx.x == 0) a.tile.scale[rt * a.tile.s_row + ct * a.tile.s_col] = fp8_scale(e);
   }
-  if (a.col.data) {
+  if (COL) {
     if (threadIdx.x < 128) {
+      // column c is half of a word for 16-bit types
+      const int c = threadIdx.x, w0 = (c >> 4) * M::kWords + (M::kHalf ? (c & 15) >> 1 : c & 15);
       uint32_t t = 0;
 #pragma unroll
-      for (int w = 0; w < 8; ++w) t = max(t, s_max[w][threadIdx.x]);
-      const uint32_t e = fp8_scale_exp(t);
-      s_max[0][threadIdx.x] = __float_as_uint(fp8_inverse(e));   // read by this thread alone before
-      const int64_t c = ct * 128 + threadIdx.x;
-      if (c < a.cols) a.col.scale[rt * a.col.s_row + c * a.col.s_col] = fp8_scale(e);
+      for (int w = 0; w < 8; ++w) t = M::larger(t, s_max[w][w0]);
+      if (M::kHalf) t = (c & 1) ? t >> 16 : t & 0xffffu;
+      const uint32_t e = fp8_scale_exp(M::bits(t));
+      s_inv[c] = fp8_inverse(e);
+      const int64_t cc = (int64_t)ct * 128 + c;
+      if (cc < a.cols) a.col.scale[rt * a.col.s_row + cc * a.col.s_col] = fp8_scale(e);
     }
     __syncthreads();
     float inv[16];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) inv[j] = __uint_as_float(s_max[0][l * 16 + j]);
+    for (int j = 0; j < 4; ++j) *(float4*)(inv + 4 * j) = *(const float4*)(s_inv + l * 16 + 4 * j);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int64_t r = rt * 128 + i * 32 + g;
+      const int64_t r = (int64_t)rt * 128 + i * 32 + g;
       float f[16];
       in[i].get(f);
+      if (special) {
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const bool bad = abs_bits(f[j]) >= kInfBits;
-        f[j] = bad ? __uint_as_float(0x7fc00000u) : f[j] * inv[j];
+        for (int j = 0; j < 16; ++j)
+          if (abs_bits(f[j]) >= kInfBits) f[j] = __uint_as_float(0x7fc00000u);
       }
-      if (r < a.rows && c0 < a.ldq) *(uint4*)(a.col.data + r * a.ldq + c0) = e4m3_16(f, 1.f, false);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) f[j] *= inv[j];
+      if (r < a.rows && c0 < a.ldq) *(uint4*)(a.col.data + r * a.ldq + c0) = e4m3_16<false>(f, 1.f);
     }
   }
 }
@@ -153,16 +171,25 @@ __global__ void __launch_bounds__(kThreads) fp8_tile_kernel(Fp8QuantArgs a, int6
 template <class T, int VEC>
 cudaError_t quant_go(const Fp8QuantArgs& a, cudaStream_t s) {
   const int64_t nkb = (a.cols + 127) / 128;
-  if (a.col.data || a.tile.data) {
+  const bool row = a.row.data, col = a.col.data, tile = a.tile.data;
+  if (col || tile) {
     const int64_t grid = (a.rows + 127) / 128 * nkb;
     if (grid >= 0x7fffffffll) return cudaErrorInvalidValue;
-    fp8_tile_kernel<T, VEC><<<(unsigned)grid, kThreads, 0, s>>>(a, nkb);
+    auto go = [&](auto kernel) { kernel<<<(unsigned)grid, kThreads, 0, s>>>(a, (uint32_t)nkb); };
+    if (row) {
+      if (col && tile) go(fp8_tile_kernel<T, VEC, true, true, true>);
+      else if (col) go(fp8_tile_kernel<T, VEC, true, true, false>);
+      else go(fp8_tile_kernel<T, VEC, true, false, true>);
+    } else {
+      if (col && tile) go(fp8_tile_kernel<T, VEC, false, true, true>);
+      else if (col) go(fp8_tile_kernel<T, VEC, false, true, false>);
+      else go(fp8_tile_kernel<T, VEC, false, false, true>);
+    }
     return cudaGetLastError();
   }
-  const bool by_rows = a.rows >= 32;
-  const int64_t items = row_items(a.rows, nkb, by_rows), grid = (items + 1) / 2;
-  if (grid >= 0x7fffffffll) return cudaErrorInvalidValue;
-  fp8_row_kernel<T, VEC, 2><<<(unsigned)grid, kThreads, 0, s>>>(a, nkb, items, by_rows);
+  const int64_t items = row_items(a.rows, nkb), grid = (items + 1) / 2;
+  if (items >= 0x7fffffffll) return cudaErrorInvalidValue;
+  fp8_row_kernel<T, VEC, 2><<<(unsigned)grid, kThreads, 0, s>>>(a, (uint32_t)nkb, (uint32_t)items);
   return cudaGetLastError();
 }
 template <class T>
@@ -172,42 +199,46 @@ cudaError_t quant_vec(const Fp8QuantArgs& a, cudaStream_t s) {
 
 // ---- decoding: 16 elements a thread
 template <class T, int VEC>
-__global__ void __launch_bounds__(kThreads) fp8_dequant_kernel(Fp8DequantArgs a, int64_t nkb, int64_t items, bool by_rows) {
+__global__ void __launch_bounds__(kThreads) fp8_dequant_kernel(Fp8DequantArgs a, uint32_t nkb) {
   constexpr int kE = (int)sizeof(typename T::elem);
+  using W = WarpSpans<T, VEC>;
+  __shared__ __align__(16) uint8_t stage[8][W::kStage];
   const int g = threadIdx.x >> 3, l = threadIdx.x & 7;
-  const RowSpan at = row_span(blockIdx.x, g, a.rows, nkb, by_rows);
-  const int64_t c0 = at.kb * 128 + l * 16;
-  if (!at.live || c0 >= a.cols) return;
-  const u128 w = load128_stream(a.data + at.row * a.ldq + c0);
-  const float* sp = a.scale + (at.row >> a.rshift) * a.s_row;
-  const int n = (int)min((int64_t)16, a.cols - c0);
+  const RowSpan at = row_span(blockIdx.x, g, a.rows, nkb);
+  const int64_t c0 = (int64_t)at.kb * 128 + l * 16;
+  const int n = at.live ? (int)min((int64_t)16, max((int64_t)0, a.cols - c0)) : 0;
+  if (VEC > 0 && n <= 0) return;   // by elements the warp works as one
   float f[16];
-  const uint4 q = make_uint4((uint32_t)w.x, (uint32_t)(w.x >> 32), (uint32_t)w.y, (uint32_t)(w.y >> 32));
-  if (a.cshift) {
-    const float sc = __ldg(sp + at.kb * a.s_col);
-    e4m3_16_to_float(q, f);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) f[i] = clamp_nan(f[i] * sc, MaxOf<T>::value);
-  } else {
-    float sc[16];
+  for (int i = 0; i < 16; ++i) f[i] = 0.f;
+  if (VEC > 0 || n > 0) {
+    const u128 w = load128_stream(a.data + at.row * a.ldq + c0);
+    const float* sp = a.scale + (at.row >> a.rshift) * a.s_row;
+    const uint4 q = make_uint4((uint32_t)w.x, (uint32_t)(w.x >> 32), (uint32_t)w.y, (uint32_t)(w.y >> 32));
+    if (a.cshift) {
+      const float sc = __ldg(sp + at.kb * a.s_col);
+      e4m3_16_to_float(q, f);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) sc[i] = i < n ? __ldg(sp + (c0 + i) * a.s_col) : 0.f;
-    e4m3_16_to_float(q, f);
+      for (int i = 0; i < 16; ++i) f[i] = clamp_nan(f[i] * sc, MaxOf<T>::value);
+    } else {
+      float sc[16];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) f[i] = clamp_nan(f[i] * sc[i], MaxOf<T>::value);
+      for (int i = 0; i < 16; ++i) sc[i] = i < n ? __ldg(sp + (c0 + i) * a.s_col) : 0.f;
+      e4m3_16_to_float(q, f);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) f[i] = clamp_nan(f[i] * sc[i], MaxOf<T>::value);
+    }
   }
   Span16<T, VEC> o;
   o.set(f);
-  o.store((uint8_t*)a.out + (at.row * a.ldo + c0) * kE, n);
+  W::store(o, (uint8_t*)a.out + (at.row * a.ldo + c0) * kE, n, stage[threadIdx.x >> 5]);
 }
 
 template <class T, int VEC>
 cudaError_t dequant_go(const Fp8DequantArgs& a, cudaStream_t s) {
-  const int64_t nkb = (a.cols + 127) / 128;
-  const bool by_rows = a.rows >= 32;
-  const int64_t items = row_items(a.rows, nkb, by_rows);
+  const int64_t nkb = (a.cols + 127) / 128, items = row_items(a.rows, nkb);
   if (items >= 0x7fffffffll) return cudaErrorInvalidValue;
-  fp8_dequant_kernel<T, VEC><<<(unsigned)items, kThreads, 0, s>>>(a, nkb, items, by_rows);
+  fp8_dequant_kernel<T, VEC><<<(unsigned)items, kThreads, 0, s>>>(a, (uint32_t)nkb);
   return cudaGetLastError();
 }
 template <class T>
