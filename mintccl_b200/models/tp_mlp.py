@@ -15,6 +15,7 @@ from typing import Optional
 
 import torch
 
+from ..ops.checkpoint8 import Saved8, silu8_backward, silu8_forward
 from ..ops.gemm import AllGatherGemm, GemmReduceScatter, gemm_dsilu, gemm_t
 
 
@@ -27,17 +28,25 @@ def _operand(t: torch.Tensor) -> torch.Tensor:
 class _MLPFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x_shard, w_up, w_down, mlp):
-        h, a = mlp.ag_gemm.call_silu(x_shard, w_up)          # [T, F/n], and silu of it
+        ctx.mlp = mlp
+        if mlp.checkpoint == "fp8":
+            # of [T, F/n] only h is kept, in 8 bits: 1.03 bytes an element instead of 4
+            a, kept = silu8_forward(mlp.ag_gemm(x_shard, w_up))
+            kept = kept.data, kept.scale
+        else:
+            h, a = mlp.ag_gemm.call_silu(x_shard, w_up)      # [T, F/n], and silu of it
+            kept = h, a
         y = mlp.gemm_rs(a, w_down)                           # [T/n, H]
-        ctx.mlp, ctx.epoch = mlp, mlp.ag_gemm.epoch
-        ctx.save_for_backward(x_shard, w_up, w_down, h, a)
+        ctx.epoch = mlp.ag_gemm.epoch
+        ctx.save_for_backward(x_shard, w_up, w_down, *kept)
         return y
 
     @staticmethod
     def backward(ctx, dy_shard):
         mlp = ctx.mlp
         comm = mlp.comm
-        x_shard, w_up, w_down, h, a = map(_operand, ctx.saved_tensors)
+        x_shard, w_up, w_down = map(_operand, ctx.saved_tensors[:3])
+        kept = ctx.saved_tensors[3:]
         n, T = comm.world_size, mlp.tokens
         dy_shard = dy_shard.contiguous()
         # all-gather dy and x over tokens (plain collectives of this library); x is still in the plan's buffer, but for this
@@ -52,7 +61,12 @@ class _MLPFunction(torch.autograd.Function):
             x = x_shard.new_empty((n, *x_shard.shape))
             comm.allgather(x, inp=x_shard)
             x = x.view(T, -1)
-        dh = gemm_dsilu(dy, w_down, h)                       # [T, F/n] = (dy @ w_down) * silu'(h)   (w_down: [H, F/n])
+        if mlp.checkpoint == "fp8":
+            da = gemm_t(dy, w_down, tb=True)                 # [T, F/n] = dy @ w_down   (w_down: [H, F/n])
+            dh, a = silu8_backward(Saved8(*kept, da.shape, da.dtype), da, act=True)
+        else:
+            h, a = map(_operand, kept)
+            dh = gemm_dsilu(dy, w_down, h)                   # the same times silu'(h)
         dw_down = gemm_t(dy, a, ta=True, tb=True)            # [H, F/n] = dy^T @ a
         dw_up = gemm_t(dh, x, ta=True, tb=True)              # [F/n, H] = dh^T @ x
         dx_shard = mlp.gemm_rs_bwd.call_transposed(dh, w_up)      # reduce_scatter(dh @ w_up)    (w_up: [F/n, H])
@@ -60,11 +74,21 @@ class _MLPFunction(torch.autograd.Function):
 
 
 class TensorParallelMLP(torch.nn.Module):
-    """``tokens`` is the global token count of a step (fixed: the fused plans own buffers of that size)."""
+    """``tokens`` is the global token count of a step (fixed: the fused plans own buffers of that size).
 
-    def __init__(self, comm, tokens: int, hidden: int, ffn: int, ncomm: Optional[int] = None, seed: int = 0):
+    ``checkpoint="fp8"`` keeps the input of the activation in 8 bits between the passes (``ops/checkpoint8.py``) and neither it
+    nor the activation in bf16: 1.03 bytes for each of ``tokens x ffn / n`` elements instead of 4.  The output is computed from
+    the input as it is, the gradients from the kept copy."""
+
+    checkpoint: Optional[str] = None
+
+    def __init__(self, comm, tokens: int, hidden: int, ffn: int, ncomm: Optional[int] = None, seed: int = 0,
+                 checkpoint: Optional[str] = None):
         super().__init__()
         n = comm.world_size
+        if checkpoint not in (None, "fp8"):
+            raise ValueError("checkpoint must be None or 'fp8'")
+        self.checkpoint = checkpoint
         if ffn % n or tokens % n:
             raise ValueError("ffn and tokens must be divisible by the world size")
         self.comm, self.tokens, self.hidden, self.ffn_local = comm, tokens, hidden, ffn // n

@@ -177,3 +177,65 @@ def test_native_checks_come_before_any_launch():
     for i, v in ((1, None), (2, 8), (7, 0), (12, 7), (13, 5), (14, 0), (16, -1), (17, 1)):
         assert L.mt_gemm_fp8(*ok[:i], v, *ok[i + 1:]) < 0, i
     assert N.last_error()
+
+
+@pytest.mark.parametrize("between", [0, 1], ids=["backward_at_once", "two_in_flight"])
+def test_mlp_of_two_ranks_with_its_activation_input_in_8_bits(between, monkeypatch):
+    """The autograd wiring on two ranks (threads; plans and GEMMs as torch expressions): gradients are those of the block with
+    the activation's input replaced by its kept copy, passed straight through."""
+    import threading
+
+    import test_cpu_tp_mlp as two
+    from mintccl_b200.models import tp_mlp
+
+    class Gather(two.FakeGather):
+        def __call__(self, x, w):
+            return self.call_silu(x, w)[0]
+
+    monkeypatch.setattr(tp_mlp, "gemm_t", lambda a, b, ta=False, tb=False: (a.t() if ta else a) @ (b if tb else b.t()))
+    g = torch.Generator().manual_seed(between)
+    N, T, H, F = two.N, two.T, two.H, two.F
+    ups, downs = torch.randn(N, F, H, generator=g), torch.randn(N, H, F, generator=g)
+    xs, dys = torch.randn(2, T, H, generator=g), torch.randn(2, T, H, generator=g)
+    used, got, errors, bus, per = [0] if between == 0 else [0, 1], {}, [], two.Bus(), T // N
+
+    def rank(r):
+        try:
+            m, rows = two.mlp_of(two.Comm(bus, r), ups[r], downs[r]), slice(r * per, (r + 1) * per)
+            assert m.checkpoint is None
+            m.checkpoint, m.ag_gemm = "fp8", Gather(m.comm)
+            shards = [xs[i][rows].clone().requires_grad_(True) for i in used]
+            outs = [m(s) for s in shards]
+            got[r] = [(y.detach(), *torch.autograd.grad(y, [s, m.w_up, m.w_down], dys[i][rows]))
+                      for i, s, y in zip(used, shards, outs)]
+        except Exception as e:
+            errors.append(e)
+            bus.bar.abort()
+
+    threads = [threading.Thread(target=rank, args=(r,)) for r in range(N)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    assert not errors, errors
+    for k, i in enumerate(used):
+        x = xs[i].clone().requires_grad_(True)
+        u, d = ups.clone().requires_grad_(True), downs.clone().requires_grad_(True)
+        h = [x @ u[r].t() for r in range(N)]
+        y = sum(torch.nn.functional.silu(h[r]) @ d[r].t() for r in range(N))
+        kept = [h[r] + (c8.save8(h[r]).restore() - h[r].detach()) for r in range(N)]
+        z = sum(torch.nn.functional.silu(kept[r]) @ d[r].t() for r in range(N))
+        dx, du, dd = torch.autograd.grad(z, [x, u, d], dys[i])
+        for r in range(N):
+            rows = slice(r * per, (r + 1) * per)
+            for a, b in zip(got[r][k], (y.detach()[rows], dx[rows], du[r], dd[r])):
+                torch.testing.assert_close(a, b, rtol=1e-4, atol=1e-4)     # fp32 sums of at most 20 terms
+
+
+def test_mlp_refuses_unknown_checkpoints():
+    from mintccl_b200.models import tp_mlp
+
+    class Comm:
+        world_size = 1
+    with pytest.raises(ValueError):
+        tp_mlp.TensorParallelMLP(Comm(), 128, 256, 256, checkpoint="fp4")

@@ -388,3 +388,59 @@ def test_activation_on_another_stream():
         got = [c8.silu8_forward(h)[0] for _ in range(5)]
     torch.cuda.synchronize()
     assert all(torch.equal(t, want) for t in got)
+
+
+# ---- the MLP block -----------------------------------------------------------------------------------------------------
+def test_mlp_with_its_activation_input_in_8_bits():
+    """Against 64 bits from the kept copy.  Roundings to bf16, half a step 2 ** -9 each (and 5 % for what is second order or
+    fp32): the activation and the output for w_down's gradient; dy @ w_down, dh and the output for the others."""
+    import mintccl_b200
+    from mintccl_b200 import Config
+    from mintccl_b200.models.tp_mlp import TensorParallelMLP
+    from mintccl_b200.parallel.rendezvous import SingleControl
+    cfg = Config.from_env(max_channels=2, num_blocks=2, buff_size=1 << 20, heap_bytes=64 << 20, scratch_bytes=1 << 20,
+                          wait_timeout_ms=4000)
+    comm = mintccl_b200.Communicator(control=SingleControl(), device=0, config=cfg)
+    T, H, F = 384, 256, 512
+    plain, mlp = TensorParallelMLP(comm, T, H, F), TensorParallelMLP(comm, T, H, F, checkpoint="fp8")
+    assert torch.equal(plain.w_up, mlp.w_up)
+    g = torch.Generator(device="cuda").manual_seed(2)
+    with torch.no_grad():
+        mlp.w_up.mul_(3.0)
+        plain.w_up.copy_(mlp.w_up)
+    x, dy, x2 = (torch.randn(T, H, generator=g, device="cuda").to(torch.bfloat16).requires_grad_(True) for _ in range(3))
+    dy = dy.detach()
+    saved = []
+
+    def pack(t):
+        saved.append(t)
+        return t
+
+    def unpack(t):      # a hook may hand a tensor back in another layout or off the 16-byte grid
+        return t.t().contiguous().t() if t.dtype is torch.uint8 else torch.cat([t.new_zeros(1), t.reshape(-1)])[1:].view(t.shape)
+
+    with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+        y, other = mlp(x), mlp(x2)      # another pass in between
+        operands = [t.data_ptr() for t in (x, x2, mlp.w_up, mlp.w_down)]
+        assert sum(t.numel() * t.element_size() for t in saved if t.data_ptr() not in operands) == 2 * T * (F + 4 * (F // 128))
+        got = torch.autograd.grad(y, [x, mlp.w_up, mlp.w_down], dy)
+    comm.check()
+    # the same output but for the last place of the activation (exponential and quotient within 1e-5)
+    want = plain(x).detach().double()
+    h = plain.ag_gemm(x.detach(), mlp.w_up.detach()).double()
+    act = (h * torch.sigmoid(h)).abs()
+    tol = (act @ mlp.w_down.detach().double().abs().t()) * 2.0 ** -8 * 1.05 + want.abs() * 2.0 ** -8 + 1e-30
+    assert bool(((y.detach().double() - want).abs() <= tol).all())
+    hk = c8.save8(h.bfloat16()).restore().double()
+    p = torch.sigmoid(hk)
+    slope = p * (1 + hk * (1 - p))
+    d, up, down, xd = dy.double(), mlp.w_up.detach().double(), mlp.w_down.detach().double(), x.detach().double()
+    dh, a, half = (d @ down) * slope, hk * p, 2.0 ** -9 * 1.05
+    for t, ref, mag in ((got[2], d.t() @ a, (d.abs().t() @ a.abs()) * half),
+                        (got[1], dh.t() @ xd, (dh.abs().t() @ xd.abs()) * 2 * half),
+                        (got[0], dh @ up, (dh.abs() @ up.abs()) * 2 * half)):
+        # dh's error is relative to dy @ w_down's rounding, not to a sum: the fp32 sums under it add 2 ** -16 of magnitudes
+        extra = 2.0 ** -16 * mag.max()
+        assert bool(((t.double() - ref).abs() <= mag + ref.abs() * half + extra).all())
+    assert other.isfinite().all()
+    comm.close()
