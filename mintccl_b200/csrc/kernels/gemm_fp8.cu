@@ -412,11 +412,11 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_fp8_kernel(const __grid_cons
 #pragma unroll
       for (int i = 0; i < CW / 2; ++i) acc[i] = 0;
       for (int kb = 0; kb < kblocks; ++kb) {
-        if (!ready && !wait_bar(&ctl->acc_full[b], bph, abort_flag, a.timeout_ns)) {
+        // one answer for all lanes
+        if (!__all_sync(0xffffffffu, ready || wait_bar(&ctl->acc_full[b], bph, abort_flag, a.timeout_ns))) {
           ok = false;
           break;
         }
-        __syncwarp();
         tc_fence_after();
         // all columns to registers, and the accumulator back to the tensor core before they are added
         const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + b * BN + half * CW;
