@@ -24,22 +24,23 @@ __device__ __forceinline__ float fp8_scale(uint32_t e) { return __uint_as_float(
 __device__ __forceinline__ float fp8_inverse(uint32_t e) { return __uint_as_float((254u - e) << 23); }   // e <= 247
 
 __device__ __forceinline__ uint32_t abs_bits(float f) { return __float_as_uint(f) & 0x7fffffffu; }
-// 16 values times inv as e4m3.  SPECIAL: some may not be finite.
-template <bool SPECIAL>
+// 16 values times inv as e4m3: finite ones or NaN.
 __device__ __forceinline__ uint4 e4m3_16(const float* f, float inv) {
   uint32_t w[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float v[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      v[j] = f[4 * i + j] * inv;
-      if (SPECIAL && abs_bits(f[4 * i + j]) >= kInfBits) v[j] = __uint_as_float(0x7fc00000u);
-    }
-    w[i] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(v[0], v[1]), __NV_SATFINITE, __NV_E4M3) |
-           ((uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(v[2], v[3]), __NV_SATFINITE, __NV_E4M3) << 16);
-  }
+  for (int i = 0; i < 4; ++i)
+    w[i] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(f[4 * i] * inv, f[4 * i + 1] * inv), __NV_SATFINITE, __NV_E4M3) |
+           ((uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(f[4 * i + 2] * inv, f[4 * i + 3] * inv), __NV_SATFINITE, __NV_E4M3) << 16);
   return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// What is not finite as NaN.  Rare: the empty statement keeps the compiler from doing it for every block and selecting after.
+__device__ __forceinline__ void only_finite16(float* f, bool special) {
+  if (special) {
+    asm volatile("");
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (abs_bits(f[i]) >= kInfBits) f[i] = __uint_as_float(0x7fc00000u);
+  }
 }
 __device__ __forceinline__ void e4m3_16_to_float(const uint4& q, float* f) {
   const uint32_t w[4] = {q.x, q.y, q.z, q.w};
@@ -247,20 +248,33 @@ struct Mags {
   }
 };
 
-// Largest finite value of a type, for restored values that rounding took past it.
+// Largest finite value of a type, for restored values that rounding took past it: 448 times a scale above `scale` (2^119,
+// 2^7 for fp16) may be.
 template <class T>
 struct MaxOf;
 template <>
-struct MaxOf<F32> { static constexpr float value = 3.4028234663852886e38f; };
+struct MaxOf<F32> { static constexpr float value = 3.4028234663852886e38f, scale = 6.646139978924579e35f; };
 template <>
-struct MaxOf<F16> { static constexpr float value = 65504.f; };
+struct MaxOf<F16> { static constexpr float value = 65504.f, scale = 128.f; };
 template <>
-struct MaxOf<BF16> { static constexpr float value = 3.3895313892515355e38f; };
+struct MaxOf<BF16> { static constexpr float value = 3.3895313892515355e38f, scale = 6.646139978924579e35f; };
 // v within +- m, NaN kept
 __device__ __forceinline__ float clamp_nan(float v, float m) {
   asm("min.NaN.f32 %0, %0, %1;" : "+f"(v) : "f"(m));
   asm("max.NaN.f32 %0, %0, %1;" : "+f"(v) : "f"(-m));
   return v;
+}
+// 16 payload values times their scale, within T's range
+template <class T>
+__device__ __forceinline__ void restore16(const u128& w, float scale, float* f) {
+  e4m3_16_to_float(make_uint4((uint32_t)w.x, (uint32_t)(w.x >> 32), (uint32_t)w.y, (uint32_t)(w.y >> 32)), f);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) f[i] *= scale;
+  if (!(fabsf(scale) <= MaxOf<T>::scale)) {
+    asm volatile("");
+#pragma unroll
+    for (int i = 0; i < 16; ++i) f[i] = clamp_nan(f[i], MaxOf<T>::value);
+  }
 }
 
 // Where a thread of the row-block kernels works: eight lanes share a block of 128, 16 elements each, and a CTA of 256
@@ -313,6 +327,7 @@ __device__ __forceinline__ bool row_tops(const Span16<T, VEC>* v, uint32_t* top)
   for (int u = 1; u < U; ++u) all = max(all, top[u]);
   const bool special = __any_sync(0xffffffffu, all >= kInfBits);
   if (special) {
+    asm volatile("");   // rare, as above
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       m.clear();
@@ -325,12 +340,11 @@ __device__ __forceinline__ bool row_tops(const Span16<T, VEC>* v, uint32_t* top)
 }
 // Encodes the 16 values of this lane as part of its row block.  All lanes of the warp take part.
 template <class T, int VEC>
-__device__ __forceinline__ uint4 encode_row16(const Span16<T, VEC>& v, const float* f, uint32_t* exp_out) {
+__device__ __forceinline__ uint4 encode_row16(const Span16<T, VEC>& v, float* f, uint32_t* exp_out) {
   uint32_t top;
-  const bool special = row_tops<T, VEC, 1>(&v, &top);
+  only_finite16(f, row_tops<T, VEC, 1>(&v, &top));
   *exp_out = fp8_scale_exp(top);
-  const float inv = fp8_inverse(*exp_out);
-  return special ? e4m3_16<true>(f, inv) : e4m3_16<false>(f, inv);
+  return e4m3_16(f, fp8_inverse(*exp_out));
 }
 
 }  // namespace mt

@@ -4,8 +4,6 @@
 // The reference has no fp8 path; it is on its roadmap (README.md:58-60).
 #include <cuda_runtime.h>
 
-#include <type_traits>
-
 #include "../device/fp8_block.cuh"
 #include "fp8.h"
 #include "launch.h"
@@ -40,7 +38,8 @@ __global__ void __launch_bounds__(kThreads) fp8_row_kernel(Fp8QuantArgs a, uint3
     float f[16];
     in[u].get(f);
     const uint32_t e = fp8_scale_exp(top[u]);
-    const uint4 q = special ? e4m3_16<true>(f, fp8_inverse(e)) : e4m3_16<false>(f, fp8_inverse(e));
+    only_finite16(f, special);
+    const uint4 q = e4m3_16(f, fp8_inverse(e));
     if (!at[u].live) continue;
     const int64_t c0 = (int64_t)at[u].kb * 128 + l * 16;
     if (c0 < a.ldq) *(uint4*)(a.row.data + at[u].row * a.ldq + c0) = q;   // the padding of a row is zeros
@@ -73,22 +72,19 @@ __global__ void __launch_bounds__(kThreads, sizeof(typename T::elem) == 2 && !RO
   if (ROW) {
     uint32_t top[4];
     const bool special = row_tops<T, VEC, 4>(in, top);
-    auto put = [&](auto SPECIAL) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int64_t r = (int64_t)rt * 128 + i * 32 + g;
-        float f[16];
-        in[i].get(f);
-        const uint32_t e = fp8_scale_exp(top[i]);
-        const uint4 q = e4m3_16<decltype(SPECIAL)::value>(f, fp8_inverse(e));
-        if (r < a.rows) {
-          if (c0 < a.ldq) *(uint4*)(a.row.data + r * a.ldq + c0) = q;
-          if (l == 0) a.row.scale[r * a.row.s_row + ct * a.row.s_col] = fp8_scale(e);
-        }
+    for (int i = 0; i < 4; ++i) {
+      const int64_t r = (int64_t)rt * 128 + i * 32 + g;
+      float f[16];
+      in[i].get(f);
+      only_finite16(f, special);
+      const uint32_t e = fp8_scale_exp(top[i]);
+      const uint4 q = e4m3_16(f, fp8_inverse(e));
+      if (r < a.rows) {
+        if (c0 < a.ldq) *(uint4*)(a.row.data + r * a.ldq + c0) = q;
+        if (l == 0) a.row.scale[r * a.row.s_row + ct * a.row.s_col] = fp8_scale(e);
       }
-    };
-    if (special) put(std::true_type());
-    else put(std::false_type());
+    }
   }
   if (!COL && !TILE) return;
   M m;
@@ -112,6 +108,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(typename T::elem) == 2 && !RO
   for (int i = 0; i < 4; ++i) m.template fold<false>(in[i].v);
   const bool special = __syncthreads_or(m.top() >= kInfBits);
   if (special) {
+    asm volatile("");
     m.clear();
 #pragma unroll
     for (int i = 0; i < 4; ++i) m.template fold<true>(in[i].v);
@@ -129,7 +126,8 @@ __global__ void __launch_bounds__(kThreads, sizeof(typename T::elem) == 2 && !RO
       const int64_t r = (int64_t)rt * 128 + i * 32 + g;
       float f[16];
       in[i].get(f);
-      const uint4 q = special ? e4m3_16<true>(f, inv) : e4m3_16<false>(f, inv);
+      only_finite16(f, special);
+      const uint4 q = e4m3_16(f, inv);
       if (r < a.rows && c0 < a.ldq) *(uint4*)(a.tile.data + r * a.ldq + c0) = q;
     }
     if (threadIdx.x == 0) a.tile.scale[rt * a.tile.s_row + ct * a.tile.s_col] = fp8_scale(e);
@@ -156,14 +154,10 @@ __global__ void __launch_bounds__(kThreads, sizeof(typename T::elem) == 2 && !RO
       const int64_t r = (int64_t)rt * 128 + i * 32 + g;
       float f[16];
       in[i].get(f);
-      if (special) {
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-          if (abs_bits(f[j]) >= kInfBits) f[j] = __uint_as_float(0x7fc00000u);
-      }
+      only_finite16(f, special);
 #pragma unroll
       for (int j = 0; j < 16; ++j) f[j] *= inv[j];
-      if (r < a.rows && c0 < a.ldq) *(uint4*)(a.col.data + r * a.ldq + c0) = e4m3_16<false>(f, 1.f);
+      if (r < a.rows && c0 < a.ldq) *(uint4*)(a.col.data + r * a.ldq + c0) = e4m3_16(f, 1.f);
     }
   }
 }
@@ -214,17 +208,13 @@ __global__ void __launch_bounds__(kThreads) fp8_dequant_kernel(Fp8DequantArgs a,
   if (VEC > 0 || n > 0) {
     const u128 w = load128_stream(a.data + at.row * a.ldq + c0);
     const float* sp = a.scale + (at.row >> a.rshift) * a.s_row;
-    const uint4 q = make_uint4((uint32_t)w.x, (uint32_t)(w.x >> 32), (uint32_t)w.y, (uint32_t)(w.y >> 32));
     if (a.cshift) {
-      const float sc = __ldg(sp + at.kb * a.s_col);
-      e4m3_16_to_float(q, f);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) f[i] = clamp_nan(f[i] * sc, MaxOf<T>::value);
+      restore16<T>(w, __ldg(sp + at.kb * a.s_col), f);
     } else {
       float sc[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) sc[i] = i < n ? __ldg(sp + (c0 + i) * a.s_col) : 0.f;
-      e4m3_16_to_float(q, f);
+      restore16<F32>(w, 1.f, f);
 #pragma unroll
       for (int i = 0; i < 16; ++i) f[i] = clamp_nan(f[i] * sc[i], MaxOf<T>::value);
     }
