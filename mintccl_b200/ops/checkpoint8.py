@@ -55,19 +55,20 @@ def _forward(h: torch.Tensor, u: Optional[torch.Tensor]):
         raise ValueError("gate and up must be of one shape, type and device")
     h2, u2 = _matrix(h), None if u is None else _matrix(u)
     if not _native(*((h2,) if u is None else (h2, u2))):
-        hf = h.detach().float()
-        y = hf / (1 + torch.exp(-hf))
-        y = (y if u is None else y * u.detach().float()).to(h.dtype)
-        return y, save8(h), None if u is None else save8(u)
+        with torch.no_grad():
+            hf = h.float()
+            y = hf / (1 + torch.exp(-hf))
+            y = (y if u is None else y * u.float()).to(h.dtype)
+            return y, save8(h), None if u is None else save8(u)
     (rows, cols), dev = h2.shape, h.device
-    hd, hs = _new_payload(rows, cols, dev), _new_scale(rows, cols, "row", dev)
-    y = torch.empty(h.shape, device=dev, dtype=h.dtype)
+    hd, hs = _new_payload(rows, cols, h2), _new_scale(rows, cols, "row", dev)
+    y = h2.new_empty(h.shape)
     h2, ldh = _rows(h2)
     if u is None:
         ud = us = None
         up = 0, 0, 0, 0
     else:
-        ud, us = _new_payload(rows, cols, dev), _new_scale(rows, cols, "row", dev)
+        ud, us = _new_payload(rows, cols, h2), _new_scale(rows, cols, "row", dev)
         u2, ldu = _rows(u2)
         up = u2.data_ptr(), ldu, ud.data_ptr(), us.data_ptr()
     if y.numel():
@@ -89,20 +90,21 @@ def _backward(h: Saved8, u: Optional[Saved8], dy: torch.Tensor, act: bool):
             raise ValueError("the saved payload does not have its tensor's shape")
         _check_scale(k.scale, _scale_shape(rows, cols, "row"), k.data, "scale")
     if not _native(dy2, *(t for k in kept for t in (k.data, k.scale))):
-        d, x = dy.detach().float(), h.restore(torch.float32)
-        p = 1 / (1 + torch.exp(-x))
-        slope, s = p * (1 + x * (1 - p)), x * p
-        v = torch.ones_like(x) if u is None else u.restore(torch.float32)
-        return (d * v * slope).to(dy.dtype), None if u is None else (d * s).to(dy.dtype), (s * v).to(dy.dtype) if act else None
+        with torch.no_grad():
+            d, x = dy.float(), h.restore(torch.float32)
+            p = 1 / (1 + torch.exp(-x))
+            slope, s = p * (1 + x * (1 - p)), x * p
+            v = torch.ones_like(x) if u is None else u.restore(torch.float32)
+            return (d * v * slope).to(dy.dtype), None if u is None else (d * s).to(dy.dtype), (s * v).to(dy.dtype) if act else None
     dy2, ld = _rows(dy2)
-    new = lambda want: torch.empty(dy.shape, device=dy.device, dtype=dy.dtype) if want else None      # noqa: E731
+    new = lambda want: dy2.new_empty(dy.shape) if want else None      # noqa: E731
     dh, du, y = new(True), new(u is not None), new(act)
     if dh.numel():
         pitch, ins, live = _up16(cols), [], []
         for k in kept:
             data, p = _payload(k.data, "the saved payload", vectors=True)
             if p != pitch:      # a copy of what was kept may come back with rows further apart
-                data = _new_payload(rows, cols, data.device).copy_(data)
+                data = _new_payload(rows, cols, data).copy_(data)
             live.append(data)
             ins += [data.data_ptr(), k.scale.data_ptr(), *k.scale.stride()]
         if u is None:

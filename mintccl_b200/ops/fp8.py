@@ -49,12 +49,6 @@ def _call(op: int, device: int, *args: int) -> None:
         raise RuntimeError(f"mt_fp8 operation {op}: {N.last_error()}")
 
 
-def _recording() -> bool:
-    """Somebody records or replaces the operations on tensors: a kernel launched from here would be missing from the record."""
-    return (torch._C._get_tracing_state() is not None or torch.compiler.is_compiling()
-            or torch._C._len_torch_dispatch_stack() != 0)
-
-
 def _address(t: torch.Tensor) -> int:
     """Where ``t`` is on a GPU, or 0: it is elsewhere, has no elements, or does not stand for its own memory (what vmap,
     functionalisation and lazy zeros make has no address or none to be asked for)."""
@@ -68,7 +62,12 @@ def _address(t: torch.Tensor) -> int:
 
 def _native(*ts: torch.Tensor) -> bool:
     """Whether kernels may be pointed at all of these; tensors without elements count."""
-    return not _recording() and all(_address(t) or _plain_cuda(t) for t in ts)
+    if torch._C._get_tracing_state() is not None or torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() != 0:
+        return False        # somebody records or replaces operations: a kernel launched from here would be missing from the record
+    for t in ts:
+        if not (_address(t) or (t.numel() == 0 and _plain_cuda(t))):
+            return False
+    return True
 
 
 def _cdiv(a: int, b: int) -> int:
@@ -84,10 +83,11 @@ def _scale_shape(rows: int, cols: int, block: str) -> Tuple[int, int]:
     return -(-rows // br), -(-cols // bc)
 
 
-def _new_payload(rows: int, cols: int, device) -> torch.Tensor:
-    """Rows a multiple of 16 bytes apart, as the kernels (and TMA) want them; the padding is not part of the result."""
-    pitch = _up16(cols)
-    buf = torch.empty((rows, pitch), device=device, dtype=torch.uint8)
+def _new_payload(rows: int, cols: int, like: torch.Tensor) -> torch.Tensor:
+    """On ``like``'s device.  Rows a multiple of 16 bytes apart, as the kernels (and TMA) want them; the padding is not part of
+    the result."""
+    pitch = (cols + 15) & ~15
+    buf = like.new_empty((rows, pitch), dtype=torch.uint8)
     return buf if pitch == cols else buf[:, :cols]
 
 
@@ -118,7 +118,7 @@ def _payload(t: torch.Tensor, name: str, vectors: bool = False) -> Tuple[torch.T
             return t, pitch
         if t.storage_offset() + (rows - 1) * pitch + _up16(cols) <= t.untyped_storage().nbytes():
             return t, pitch
-    buf = _new_payload(rows, cols, t.device)
+    buf = _new_payload(rows, cols, t)
     buf.copy_(t.view(torch.uint8))
     return buf, _up16(cols)
 
@@ -138,6 +138,15 @@ def _check_float(x: torch.Tensor, name: str) -> None:
 def quantize_fp8(x: torch.Tensor, block: str = "row") -> Quantized:
     """fp32 / fp16 / bf16 ``[rows, cols]`` -> (payload uint8 ``[rows, cols]``, scales).  Payload rows are a multiple of 16
     bytes apart; the scales of row blocks are held with neighbouring rows adjacent (strides ``(1, rows)``)."""
+    if block == "row" and x.dim() == 2 and x.dtype in DTYPES and _native(x):    # as below, for the small calls of a decode step
+        rows, cols = x.shape
+        kb = -(-cols // BLOCK)
+        data, scale = _new_payload(rows, cols, x), torch.empty_strided((rows, kb), (1, rows), device=x.device, dtype=torch.float32)
+        if rows and cols:
+            x, ld = _rows(x)
+            _call(QUANTIZE, x.get_device(), DTYPES[x.dtype], x.data_ptr(), ld, rows, cols, (cols + 15) & ~15, data.data_ptr(),
+                  scale.data_ptr(), 0, 0, 0, 0)
+        return data, scale
     return quantize_fp8_many(x, (block,))[0]
 
 
@@ -151,7 +160,7 @@ def quantize_fp8_many(x: torch.Tensor, blocks: Sequence[str]) -> List[Quantized]
     if not _native(x):
         return [_torch_quantize(x, b) for b in blocks]
     rows, cols = x.shape
-    out = {b: (_new_payload(rows, cols, x.device), _new_scale(rows, cols, b, x.device)) for b in blocks}
+    out = {b: (_new_payload(rows, cols, x), _new_scale(rows, cols, b, x.device)) for b in blocks}
     if x.numel():
         x, ld = _rows(x)
         ptrs = [0] * 6
@@ -180,7 +189,7 @@ def _torch_quantize(x: torch.Tensor, block: str) -> Quantized:
     e = torch.where(m > 0.875, e - 8, e - 9).clamp(min=-126)      # 448 = 0.875 * 2 ** 9
     scale = torch.where(m > 0, ((e + 127) << 23).view(torch.float32), torch.ones_like(m))
     q = torch.where(finite, x / _spread(scale, rows, cols, block), torch.full_like(x, float("nan"))).to(torch.float8_e4m3fn)
-    data = _new_payload(rows, cols, x.device).copy_(q.view(torch.uint8))
+    data = _new_payload(rows, cols, x).copy_(q.view(torch.uint8))
     return data, (scale.t().contiguous().t() if block == "row" else scale)
 
 
@@ -197,7 +206,7 @@ def dequantize_fp8(data: torch.Tensor, scale: torch.Tensor, block: str = "row", 
     if not _native(data, scale):
         top = torch.finfo(dtype).max
         return (data.view(torch.float8_e4m3fn).float() * _spread(scale, rows, cols, block)).clamp(-top, top).to(dtype)
-    out = torch.empty((rows, cols), device=data.device, dtype=dtype)
+    out = data.new_empty((rows, cols), dtype=dtype)
     if out.numel():
         data, pitch = _payload(data, "data", vectors=True)
         br, bc = BLOCKS[block]
@@ -236,7 +245,7 @@ def gemm_fp8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: t
     if out is None:
         if dtype not in DTYPES:
             raise ValueError("dtype must be float32, float16 or bfloat16")
-        out, ldc = torch.empty((M, Nn), device=device, dtype=dtype), Nn
+        out, ldc = a.new_empty((M, Nn), dtype=dtype), Nn
     else:
         ldc = out.stride(0) if out.dim() == 2 and M > 1 else Nn
         if (tuple(out.shape) != (M, Nn) or out.dtype not in DTYPES or out.device != device or not _native(out)
@@ -305,6 +314,8 @@ class _LinearFp8(torch.autograd.Function):
         kept, w_data, w_scale = ctx.saved_tensors
         t, n, k, offs, size, x_dtype, w_dtype = ctx.sizes
         want_x, want_w = ctx.needs_input_grad[:2]
+        if not _native(dy):
+            raise ValueError("the gradient must be a plain CUDA tensor, and nobody recording")
         base = 0
         if size:   # what a saved-tensor hook made of it
             kept = kept.contiguous()

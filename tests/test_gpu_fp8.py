@@ -74,7 +74,7 @@ def operands(form, M, N, K, seed=0, spread=1.0):
     g = torch.Generator(device="cuda").manual_seed(seed + M + 3 * N + 5 * K)
 
     def one(rows, cols, block):
-        data = fp8._new_payload(rows, cols, "cuda")
+        data = fp8._new_payload(rows, cols, torch.empty(0, device="cuda"))
         v = (torch.randn(rows, cols, generator=g, device="cuda") * 100).clamp(-448, 448)
         data.copy_(v.to(torch.float8_e4m3fn).view(torch.uint8))
         scale = fp8._new_scale(rows, cols, block, "cuda")
@@ -444,3 +444,105 @@ def test_mlp_with_its_activation_input_in_8_bits():
         assert bool(((t.double() - ref).abs() <= mag + ref.abs() * half + extra).all())
     assert other.isfinite().all()
     comm.close()
+
+
+# ---- calls that the documentation allows ------------------------------------------------------------------------------
+def test_layer_takes_vectors_and_strided_operands():
+    g = torch.Generator(device="cuda").manual_seed(3)
+    w = torch.randn(96, 160, generator=g, device="cuda", dtype=torch.bfloat16)
+    x = torch.randn(7, 320, generator=g, device="cuda", dtype=torch.bfloat16)
+    assert torch.equal(fp8.linear_fp8(x[0, :160], w), fp8.linear_fp8(x[:1, :160].contiguous(), w)[0])
+    for xs, ws in ((x[:, ::2], w), (x[:, 1:161], w.t().contiguous().t()), (x[::3, 160:], w), (x[:1, :160].expand(5, 160), w[::2])):
+        a = [t.detach().requires_grad_(True) for t in (xs, ws)]
+        b = [t.detach().contiguous().clone().requires_grad_(True) for t in (xs, ws)]
+        ya, yb = fp8.linear_fp8(*a), fp8.linear_fp8(*b)
+        dy = torch.randn(ya.shape, generator=g, device="cuda").bfloat16()
+        assert torch.equal(ya, yb)
+        for p, q in zip(torch.autograd.grad(ya, a, dy), torch.autograd.grad(yb, b, dy)):
+            assert torch.equal(p, q)
+    # gradients that are expanded or strided
+    y = fp8.linear_fp8(x[:, :160].detach().requires_grad_(True), w)
+    y.sum().backward()
+
+
+def test_layer_refuses_what_it_cannot_follow():
+    x = torch.randn(4, 64, device="cuda", requires_grad=True)
+    w = torch.randn(32, 64, device="cuda", requires_grad=True)
+    y = fp8.linear_fp8(x, w)
+    with pytest.raises(Exception):      # batched gradients have no address
+        torch.autograd.grad(y, (x, w), torch.ones(3, 4, 32, device="cuda"), is_grads_batched=True)
+    (dx,) = torch.autograd.grad(fp8.linear_fp8(x, w), x, torch.ones(4, 32, device="cuda"), create_graph=True)
+    with pytest.raises(RuntimeError):
+        dx.sum().backward()
+    from torch.fx.experimental.proxy_tensor import make_fx
+    with pytest.raises(ValueError):
+        make_fx(lambda t: fp8.linear_fp8(t, w.detach()))(x.detach())
+    q = fp8.quantize_fp8(x.detach())
+    with pytest.raises(ValueError):
+        make_fx(lambda t: fp8.gemm_fp8(t, q[1], *fp8.quantize_fp8(w.detach(), "tile")))(q[0])
+
+
+def test_traced_encoding_replays_on_other_inputs():
+    """A recorded graph of the encoding holds the operations: it gives other inputs their own bytes."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x, y = torch.randn(2, 130, 300, device="cuda")
+    for block in fp8.BLOCKS:
+        for a, b in zip(make_fx(lambda t: fp8.quantize_fp8(t, block))(x)(y), fp8.quantize_fp8(y, block)):
+            assert torch.equal(a, b)
+    h = make_fx(lambda t: c8.silu8_forward(t)[0])(x)(y)
+    torch.testing.assert_close(h, torch.nn.functional.silu(y), rtol=2.0 ** -20, atol=2.0 ** -24)
+
+
+def test_batched_gradients_of_the_activation():
+    h = torch.randn(5, 200, device="cuda", requires_grad=True)
+    d = torch.randn(3, 5, 200, device="cuda")
+    y = c8.silu8(h)
+    (got,) = torch.autograd.grad(y, h, d, is_grads_batched=True, retain_graph=True)
+    for i in range(3):
+        (want,) = torch.autograd.grad(y, h, d[i], retain_graph=True)
+        torch.testing.assert_close(got[i], want, rtol=2.0 ** -18, atol=2.0 ** -20)
+
+
+def test_first_calls_of_a_process_may_be_captured():
+    """Nothing is set up outside the capture: a new process whose first use of the kernels is inside a graph."""
+    import subprocess
+    import sys
+    code = """
+import torch
+from mintccl_b200.ops import checkpoint8 as c8, fp8
+x, w = torch.randn(300, 512, device="cuda"), torch.randn(2000, 512, device="cuda")
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    y = c8.silu8_forward(fp8.gemm_fp8(*fp8.quantize_fp8(x), *fp8.quantize_fp8(w, "tile"), dtype=torch.float32))[1].restore()
+g.replay()
+torch.cuda.synchronize()
+z = c8.silu8_forward(fp8.gemm_fp8(*fp8.quantize_fp8(x), *fp8.quantize_fp8(w, "tile"), dtype=torch.float32))[1].restore()
+assert torch.equal(y, z)
+print("same")
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120,
+                       cwd=str(N.lib_path().parents[2]))
+    assert r.returncode == 0 and "same" in r.stdout, r.stderr[-2000:]
+
+
+def test_layers_on_two_streams_at_once():
+    g = torch.Generator(device="cuda").manual_seed(9)
+    sets = []
+    for t, k, n in ((300, 512, 1000), (37, 1000, 640)):
+        x = torch.randn(t, k, generator=g, device="cuda", dtype=torch.bfloat16).requires_grad_(True)
+        w = (torch.randn(n, k, generator=g, device="cuda") * 0.05).bfloat16().requires_grad_(True)
+        dy = torch.randn(t, n, generator=g, device="cuda", dtype=torch.bfloat16)
+        y = fp8.linear_fp8(x, w)
+        sets.append((x, w, dy, (y.detach(), *torch.autograd.grad(y, (x, w), dy))))
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(8):
+        for i, (x, w, dy, _) in enumerate(sets):
+            with torch.cuda.stream(streams[i]):
+                y = fp8.linear_fp8(x, w)
+                got[i].append((y.detach(), *torch.autograd.grad(y, (x, w), dy)))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for r in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(r, sets[i][3]))
