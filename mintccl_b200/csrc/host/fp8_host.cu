@@ -163,9 +163,9 @@ int mt_fp8_act_backward(void* stream, int dtype, int64_t ldq, const void* h_data
   });
 }
 
-int mt_gemm_fp8(void* stream, const void* A, int64_t lda, const void* sa, int64_t sa_m, int64_t sa_k, const void* B, int64_t ldb,
+static int gemm(void* stream, const void* A, int64_t lda, const void* sa, int64_t sa_m, int64_t sa_k, const void* B, int64_t ldb,
                 const void* sb, int64_t sb_n, int64_t sb_k, void* C, int64_t ldc, int dtype, int64_t M, int64_t N, int64_t K,
-                int ta, int tb, int nctas) {
+                int ta, int tb, int nctas, bool pow2) {
   return guarded([&]() -> int {
     if (M <= 0 || N <= 0 || K <= 0 || M > 0x7fff0000ll || N > 0x7fff0000ll || K > 0x7fff0000ll) return fail("bad GEMM shape");
     if (ta && !tb) return fail("ta goes with tb");
@@ -203,11 +203,17 @@ int mt_gemm_fp8(void* stream, const void* A, int64_t lda, const void* sa, int64_
     a.timeout_ns = 4000000000ull;
     const int units = pair ? sms / 2 : sms, used = (int)(tiles < units ? tiles : units);
     const int grid = pair ? 2 * used : split > 1 ? split * (int)tiles : used;
-    if (launched(mt::launch_fp8_gemm(pair, split, ta != 0, tb != 0, a, grid, (cudaStream_t)stream), "fp8 gemm"))
+    if (launched(mt::launch_fp8_gemm(pair, pow2, split, ta != 0, tb != 0, a, grid, (cudaStream_t)stream), "fp8 gemm"))
       return -1;
     mthost::stat_add(mthost::ST_GEMM, (uint64_t)(2.0 * M * N * K));
     return 0;
   });
+}
+
+int mt_gemm_fp8(void* stream, const void* A, int64_t lda, const void* sa, int64_t sa_m, int64_t sa_k, const void* B, int64_t ldb,
+                const void* sb, int64_t sb_n, int64_t sb_k, void* C, int64_t ldc, int dtype, int64_t M, int64_t N, int64_t K,
+                int ta, int tb, int nctas) {
+  return gemm(stream, A, lda, sa, sa_m, sa_k, B, ldb, sb, sb_n, sb_k, C, ldc, dtype, M, N, K, ta, tb, nctas, false);
 }
 
 int mt_fp8_packed(void* stream, int op, const int64_t* v) {
@@ -224,13 +230,13 @@ int mt_fp8_packed(void* stream, int op, const int64_t* v) {
       return mt_fp8_act_backward(stream, (int)v[0], v[1], p(2), p(3), v[4], v[5], p(6), p(7), v[8], v[9], p(10), v[11], v[12], v[13],
                                  p(14), p(15), p(16));
     case MT_FP8_GEMM:
-      return mt_gemm_fp8(stream, p(0), v[1], p(2), v[3], v[4], p(5), v[6], p(7), v[8], v[9], p(10), v[11], (int)v[12], v[13], v[14],
-                         v[15], (int)v[16], (int)v[17], (int)v[18]);
+      return gemm(stream, p(0), v[1], p(2), v[3], v[4], p(5), v[6], p(7), v[8], v[9], p(10), v[11], (int)v[12], v[13], v[14], v[15],
+                  (int)v[16], (int)v[17], (int)v[18], v[19] != 0);
     case MT_FP8_LINEAR_FORWARD: {
       const int64_t T = v[3], K = v[4], N = v[8], ldq = (K + 15) / 16 * 16;
       if (mt_fp8_quantize(stream, (int)v[0], p(1), v[2], T, K, ldq, p(9), p(10), nullptr, nullptr, p(11), p(12))) return -1;
       if (v[6] && mt_fp8_quantize(stream, (int)v[5], p(6), v[7], N, K, v[14], nullptr, nullptr, nullptr, nullptr, p(13), p(15))) return -1;
-      return mt_gemm_fp8(stream, p(9), ldq, p(10), 1, T, p(13), v[14], p(15), v[16], v[17], p(18), N, (int)v[0], T, N, K, 0, 0, 0);
+      return gemm(stream, p(9), ldq, p(10), 1, T, p(13), v[14], p(15), v[16], v[17], p(18), N, (int)v[0], T, N, K, 0, 0, 0, true);
     }
     case MT_FP8_LINEAR_BACKWARD: {
       const int64_t T = v[3], N = v[4], K = v[5], ldq = (N + 15) / 16 * 16, ldx = (K + 15) / 16 * 16;
@@ -238,10 +244,9 @@ int mt_fp8_packed(void* stream, int op, const int64_t* v) {
       if (mt_fp8_quantize(stream, (int)v[0], p(1), v[2], T, N, ldq, want_x ? p(6) : nullptr, want_x ? p(7) : nullptr,
                           want_w ? p(14) : nullptr, want_w ? p(15) : nullptr, nullptr, nullptr))
         return -1;
-      if (want_x && mt_gemm_fp8(stream, p(6), ldq, p(7), 1, T, p(8), v[9], p(10), v[12], v[11], p(13), K, (int)v[0], T, K, N, 0, 1, 0))
+      if (want_x && gemm(stream, p(6), ldq, p(7), 1, T, p(8), v[9], p(10), v[12], v[11], p(13), K, (int)v[0], T, K, N, 0, 1, 0, true))
         return -1;
-      if (want_w && mt_gemm_fp8(stream, p(14), ldq, p(15), 1, N, p(16), ldx, p(17), 1, (K + 127) / 128, p(18), K, (int)v[19], N, K, T, 1,
-                                1, 0))
+      if (want_w && gemm(stream, p(14), ldq, p(15), 1, N, p(16), ldx, p(17), 1, (K + 127) / 128, p(18), K, (int)v[19], N, K, T, 1, 1, 0, true))
         return -1;
       return 0;
     }

@@ -16,6 +16,10 @@
 // and adds up its share of the tile's rows from all of them, in the order of the blocks: the same bits every time.  (Sending
 // them instead, with stores or bulk copies to the other CTAs' shared memory, took 1 - 2 us longer for 128 rows.)
 //
+// POW2 (with PAIR): the caller says that all scales are powers of two, as this library's own encoding makes them.  Then the
+// tensor core applies them itself (kind::mxf8f6f4, a scale byte for each 32 elements: four alike) and adds up a whole tile;
+// a scale that is not one counts as NaN.
+//
 //   warps 0..7   sums: a thread has one row and half of the tile's columns; then they store C
 //   warp 8       TMA producer: own halves of A and B; the bytes of both CTAs count on the leader's "stage full" barrier
 //   warp 9       (leader) issues tcgen05.mma: four a stage; commits to "stage empty" and "accumulator full" of both CTAs
@@ -51,14 +55,15 @@ constexpr int kPitch = 144;         // bytes of a staged row of C: 128 and paddi
 constexpr int kSumPitch = 132;      // floats of a row of sums in shared memory
 constexpr uint32_t A_BYTES = BM * BK, TMEM_COLS = 512;
 
-template <int BN, bool PAIR>
+template <int BN, bool PAIR, bool POW2 = false>
 struct Shape {
   static constexpr int BNC = PAIR ? BN / 2 : BN;          // rows of B staged by a CTA
   static constexpr uint32_t B_BYTES = BNC * BK;
   static constexpr int STAGES = PAIR ? 7 : 5;
-  static constexpr int ACC = TMEM_COLS / BN;              // accumulators
+  static constexpr uint32_t SF_BYTES = 1024;              // POW2: scale bytes of a stage, A's rows and B's
+  static constexpr int ACC = POW2 ? 2 : TMEM_COLS / BN;   // accumulators (POW2: the columns behind them hold scales)
   static constexpr uint32_t OPERANDS = STAGES * (A_BYTES + B_BYTES);
-  static constexpr uint32_t RING = kScaleSlots * 2 * BM * 4, STAGING = kSumWarps * 32 * kPitch;
+  static constexpr uint32_t RING = POW2 ? STAGES * SF_BYTES : kScaleSlots * 2 * BM * 4, STAGING = kSumWarps * 32 * kPitch;
   static constexpr uint32_t SMEM = 1024 + OPERANDS + RING + STAGING + 256;
   static_assert(SMEM <= 232448, "shared memory of one CTA");
   static_assert(PAIR || OPERANDS >= BM * kSumPitch * 4, "the sums of a split tile are left where the stages were");
@@ -181,9 +186,17 @@ __device__ __forceinline__ void store_split(const Fp8GemmArgs& a, uint32_t sums,
   else store_split<T, 8>(a, sums, rank, row0, col0);
 }
 
-template <int BN, bool PAIR, bool TA, bool TB>
+// The ue8m0 byte of a power of two, four times; NaN for anything else.
+__device__ __forceinline__ uint32_t scale_byte4(float s) {
+  const uint32_t b = __float_as_uint(s), e = b >> 23;
+  return ((b & 0x7fffffu) == 0 && e - 1u < 254u ? e : 255u) * 0x01010101u;
+}
+
+template <int BN, bool PAIR, bool POW2, bool TA, bool TB>
 __global__ void __launch_bounds__(kThreads, 1) gemm_fp8_kernel(const __grid_constant__ Fp8GemmArgs a) {
-  using S = Shape<BN, PAIR>;
+  static_assert(PAIR || !POW2, "the tensor core applies scales on pairs");
+  static_assert(!POW2 || Shape<BN, PAIR, POW2>::ACC * BN + Shape<BN, PAIR, POW2>::STAGES * 8 <= TMEM_COLS, "columns of TMEM");
+  using S = Shape<BN, PAIR, POW2>;
   constexpr int STAGES = S::STAGES, ACC = S::ACC, BNC = S::BNC, CW = BN / 2;   // CW: columns of a sum thread
   constexpr uint32_t B_BYTES = S::B_BYTES;
   constexpr int kRows = PAIR ? 2 * BM : BM;   // of a tile
@@ -287,7 +300,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_fp8_kernel(const __grid_cons
       }
     } else if (warp == kSumWarps + 1 && cr == 0) {
       // ---------------------------------------------------------- MMA issuer: uniform, one lane issues
-      constexpr uint32_t idesc = make_idesc_e4m3(kRows, BN) | (TA ? kIdescTransA : 0u) | (TB ? kIdescTransB : 0u);
+      constexpr uint32_t trans = (TA ? kIdescTransA : 0u) | (TB ? kIdescTransB : 0u), idesc = make_idesc_e4m3(kRows, BN) | trans;
       // a step of 32 along K: 32 bytes of a row, or 32 rows of 128 bytes
       constexpr uint64_t step_a = TA ? 256 : 2, step_b = !TB ? 2 : BNC == 128 ? 256 : 128;
       uint32_t s = 0, ph = 0, b = 0, bph = 0;
@@ -298,10 +311,12 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_fp8_kernel(const __grid_cons
       };
       for (int t = first; ok && t < tiles; t += step) {
         for (int kb = 0; kb < kblocks; ++kb) {
+          // an accumulator is one block's, with POW2 a whole tile's
+          const bool fresh = !POW2 || kb == 0, done = !POW2 || kb + 1 == kblocks;
           // both probes in flight at once: each takes some 230 cycles beside the tensor core's own shared-memory traffic
-          const bool drained = mbar_test(&ctl->acc_empty[b], bph ^ 1), loaded = mbar_test(&ctl->full[s], ph);
+          const bool drained = !fresh || mbar_test(&ctl->acc_empty[b], bph ^ 1), loaded = mbar_test(&ctl->full[s], ph);
           if (!__all_sync(0xffffffffu, drained && loaded) &&
-              (!wait_bar_warp(&ctl->acc_empty[b], bph ^ 1, abort_flag, a.timeout_ns) ||
+              ((fresh && !wait_bar_warp(&ctl->acc_empty[b], bph ^ 1, abort_flag, a.timeout_ns)) ||
                !wait_bar_warp(&ctl->full[s], ph, abort_flag, a.timeout_ns))) {
             ok = false;
             break;
@@ -312,20 +327,31 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_fp8_kernel(const __grid_cons
                               : BNC == 128 ? make_smem_desc_mn_sw128(sB + s * B_BYTES, 128 * BK)
                                            : make_smem_desc_mn_sw64(sB + s * B_BYTES);
           if (elect_one()) {
+            if constexpr (POW2) {
+              const uint32_t sfa = tmem_base + ACC * BN + s * 8, sfb = sfa + 4;
+              const uint8_t* sf = (const uint8_t*)sScale + s * S::SF_BYTES;
+              tmem_cp_sf_pair(sfa, make_smem_desc_sf(sf));
+              tmem_cp_sf_pair(sfb, make_smem_desc_sf(sf + 512));
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              if (PAIR) umma_f8_pair(tmem_base + b * BN, da + k * step_a, db + k * step_b, idesc, k > 0 ? 1u : 0u);
-              else umma_f8(tmem_base + b * BN, da + k * step_a, db + k * step_b, idesc, k > 0 ? 1u : 0u);
+              for (int k = 0; k < 4; ++k)
+                umma_mxfp8_pair(tmem_base + b * BN, da + k * step_a, db + k * step_b, make_idesc_mxfp8(kRows, BN, k, k) | trans, sfa, sfb,
+                                kb > 0 || k > 0 ? 1u : 0u);
+            } else {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                if (PAIR) umma_f8_pair(tmem_base + b * BN, da + k * step_a, db + k * step_b, idesc, k > 0 ? 1u : 0u);
+                else umma_f8(tmem_base + b * BN, da + k * step_a, db + k * step_b, idesc, k > 0 ? 1u : 0u);
+              }
             }
             commit(&ctl->empty[s]);
-            commit(&ctl->acc_full[b]);
+            if (done) commit(&ctl->acc_full[b]);
           }
           __syncwarp();
           if (++s == STAGES) {
             s = 0;
             ph ^= 1;
           }
-          if (++b == ACC) {
+          if (done && ++b == ACC) {
             b = 0;
             bph ^= 1;
           }
@@ -342,7 +368,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_fp8_kernel(const __grid_cons
       // ---------------------------------------------------------- scales: one warp for even blocks, one for odd; a lane has
       // four rows, 32 apart.  They count on the stage's "full" barrier: whoever sees the block's accumulator sees them too.
       // A slot is free when its stage is: the sums are at most ACC + STAGES blocks behind.
-      static_assert(ACC + STAGES < kScaleSlots, "slots of the scales");
+      static_assert(POW2 || ACC + STAGES < kScaleSlots, "slots of the scales");
       const int w = warp - kSumWarps - 2;
       const uint32_t full_leader = map_to_cta(smem_u32(&ctl->full[0]), 0);
       uint32_t s = w, ph = 0, pos = 0;   // stage of this warp's next block, and the tile's first block among all
@@ -370,11 +396,20 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_fp8_kernel(const __grid_cons
           for (int j = 0; j < 2; ++j) {
             if (!ok || kb + 2 * j >= kblocks) continue;
             ok = wait_bar_warp(&ctl->empty[s], ph ^ 1, abort_flag, a.timeout_ns);
-            float* f = sScale + ((pos + kb + 2 * j) & (kScaleSlots - 1)) * (2 * BM) + lane;
+            if constexpr (POW2) {
+              // byte (r % 32) * 16 + (r / 32) * 4 + k of an atom is row r's scale of the k-th 32 elements
+              uint4* sf = (uint4*)((uint8_t*)sScale + s * S::SF_BYTES) + lane;
+              const uint32_t eb = scale_byte4(vb[j][0]);
+              sf[0] = make_uint4(scale_byte4(va[j][0]), scale_byte4(va[j][1]), scale_byte4(va[j][2]), scale_byte4(va[j][3]));
+              sf[32] = make_uint4(eb, eb, eb, eb);
+              fence_proxy_async_smem();
+            } else {
+              float* f = sScale + ((pos + kb + 2 * j) & (kScaleSlots - 1)) * (2 * BM) + lane;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              f[32 * i] = va[j][i] * vb[j][0];
-              f[BM + 32 * i] = va[j][i] * vb[j][1];
+              for (int i = 0; i < 4; ++i) {
+                f[32 * i] = va[j][i] * vb[j][0];
+                f[BM + 32 * i] = va[j][i] * vb[j][1];
+              }
             }
             __syncwarp();
             if (lane == 0) {
@@ -411,7 +446,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_fp8_kernel(const __grid_cons
       uint64_t acc[CW / 2];
 #pragma unroll
       for (int i = 0; i < CW / 2; ++i) acc[i] = 0;
-      for (int kb = 0; kb < kblocks; ++kb) {
+      for (int kb = 0; kb < (POW2 ? 1 : kblocks); ++kb) {
         // one answer for all lanes
         if (!__all_sync(0xffffffffu, ready || wait_bar(&ctl->acc_full[b], bph, abort_flag, a.timeout_ns))) {
           ok = false;
@@ -424,7 +459,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_fp8_kernel(const __grid_cons
         uint32_t r[CW / 32][32];
 #pragma unroll
         for (int c = 0; c < CW / 32; ++c) tmem_ld_32x32(taddr + c * 32, r[c]);
-        const uint32_t f = __float_as_uint(factor[(pos++ & (kScaleSlots - 1)) * (2 * BM)]);
+        const uint32_t f = POW2 ? 0u : __float_as_uint(factor[(pos++ & (kScaleSlots - 1)) * (2 * BM)]);
         const uint64_t f2 = pack2(f, f);
         tmem_ld_wait();
         tc_fence_before();
@@ -437,7 +472,10 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_fp8_kernel(const __grid_cons
 #pragma unroll
         for (int c = 0; c < CW / 32; ++c)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) fma2(acc[c * 16 + i], pack2(r[c][2 * i], r[c][2 * i + 1]), f2);
+          for (int i = 0; i < 16; ++i) {
+            if (POW2) acc[c * 16 + i] = pack2(r[c][2 * i], r[c][2 * i + 1]);
+            else fma2(acc[c * 16 + i], pack2(r[c][2 * i], r[c][2 * i + 1]), f2);
+          }
         b = bn;
         bph = bphn;
       }
@@ -483,9 +521,9 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_fp8_kernel(const __grid_cons
   }
 }
 
-template <int BN, bool PAIR, bool TA, bool TB>
+template <int BN, bool PAIR, bool POW2, bool TA, bool TB>
 cudaError_t go(const Fp8GemmArgs& a, int cluster, int nctas, cudaStream_t s) {
-  const void* fn = (const void*)gemm_fp8_kernel<BN, PAIR, TA, TB>;
+  const void* fn = (const void*)gemm_fp8_kernel<BN, PAIR, POW2, TA, TB>;
   static std::atomic<uint64_t> ready{0};   // devices on which the kernel has been looked over and given its shared memory
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -495,13 +533,13 @@ cudaError_t go(const Fp8GemmArgs& a, int cluster, int nctas, cudaStream_t s) {
     cudaFuncAttributes at;
     if ((e = cudaFuncGetAttributes(&at, fn)) != cudaSuccess) return e;
     if (at.numRegs < kRegsLaunch) return cudaErrorLaunchOutOfResources;   // the register split would wait forever for what is missing
-    if ((e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<BN, PAIR>::SMEM)) != cudaSuccess) return e;
+    if ((e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<BN, PAIR, POW2>::SMEM)) != cudaSuccess) return e;
     if (dev <= 63) ready.fetch_or(bit, std::memory_order_release);
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(nctas);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = Shape<BN, PAIR>::SMEM;
+  cfg.dynamicSmemBytes = Shape<BN, PAIR, POW2>::SMEM;
   cfg.stream = s;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -509,20 +547,21 @@ cudaError_t go(const Fp8GemmArgs& a, int cluster, int nctas, cudaStream_t s) {
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, gemm_fp8_kernel<BN, PAIR, TA, TB>, a);
+  return cudaLaunchKernelEx(&cfg, gemm_fp8_kernel<BN, PAIR, POW2, TA, TB>, a);
 }
-template <int BN, bool PAIR>
+template <int BN, bool PAIR, bool POW2>
 cudaError_t go_form(bool ta, bool tb, const Fp8GemmArgs& a, int cluster, int nctas, cudaStream_t s) {
-  if (ta) return go<BN, PAIR, true, true>(a, cluster, nctas, s);
-  return tb ? go<BN, PAIR, false, true>(a, cluster, nctas, s) : go<BN, PAIR, false, false>(a, cluster, nctas, s);
+  if (ta) return go<BN, PAIR, POW2, true, true>(a, cluster, nctas, s);
+  return tb ? go<BN, PAIR, POW2, false, true>(a, cluster, nctas, s) : go<BN, PAIR, POW2, false, false>(a, cluster, nctas, s);
 }
 
 }  // namespace fp8g
 
-cudaError_t launch_fp8_gemm(bool pair, int split, bool ta, bool tb, const Fp8GemmArgs& a, int nctas, cudaStream_t s) {
+cudaError_t launch_fp8_gemm(bool pair, bool pow2, int split, bool ta, bool tb, const Fp8GemmArgs& a, int nctas, cudaStream_t s) {
   if ((ta && !tb) || split < 1 || (pair && split > 1)) return cudaErrorInvalidValue;
   count_launch();
-  return pair ? fp8g::go_form<128, true>(ta, tb, a, 2, nctas, s) : fp8g::go_form<128, false>(ta, tb, a, split, nctas, s);
+  if (pair) return pow2 ? fp8g::go_form<128, true, true>(ta, tb, a, 2, nctas, s) : fp8g::go_form<128, true, false>(ta, tb, a, 2, nctas, s);
+  return fp8g::go_form<128, false, false>(ta, tb, a, split, nctas, s);
 }
 
 int fp8_gemm_error() {

@@ -178,7 +178,8 @@ int mt_fp8_act_backward(void* stream, int dtype, int64_t ldq, const void* h_data
 int mt_gemm_fp8(void* stream, const void* A, int64_t lda, const void* sa, int64_t sa_m, int64_t sa_k, const void* B, int64_t ldb,
                 const void* sb, int64_t sb_n, int64_t sb_k, void* C, int64_t ldc, int dtype, int64_t M, int64_t N, int64_t K,
                 int ta, int tb, int nctas);
-// The functions above with their arguments after `stream` as 64-bit integers (ctypes takes 3 us to convert twenty
+// The functions above with their arguments after `stream` as 64-bit integers (MT_FP8_GEMM has one more: all scales are
+// powers of two, and what is not counts as NaN; ctypes takes 3 us to convert twenty
 // arguments one by one), and the two passes of a linear layer, each of them all of its kernels in one call.
 //   MT_FP8_LINEAR_FORWARD   dtype, x, ldx, T, K, w_dtype, w (0: encoded already), ldw, N, xr_data, xr_scale, xt_data, xt_scale
 //                           (both 0: not wanted), w_data, ldwq, w_scale, w_srow, w_scol, y

@@ -217,14 +217,17 @@ def dequantize_fp8(data: torch.Tensor, scale: torch.Tensor, block: str = "row", 
 
 # ---- products ------------------------------------------------------------------------------------------------------
 def gemm_fp8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor, ta: bool = False, tb: bool = False,
-             out: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.bfloat16, nctas: int = 0) -> torch.Tensor:
+             out: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.bfloat16, nctas: int = 0,
+             power_of_two: bool = False) -> torch.Tensor:
     """``op(a) @ op(b)`` of quantised matrices as they are stored, any sizes (kernel: ``csrc/kernels/gemm_fp8.cu``):
 
     * ``a [M, K] @ b[N, K].T``: a layer's output; ``a`` in row blocks, ``b`` (the weight) in tiles;
     * ``tb``: ``a [M, K] @ b [K, N]``: the gradient of its input; ``a`` in row blocks, ``b`` in tiles;
     * ``ta`` and ``tb``: ``a[K, M].T @ b [K, N]``: the gradient of its weight; ``a`` in column blocks, ``b`` in tiles.
 
-    Sums are fp32 with one rounding to ``dtype`` (fp32, fp16 or bf16; that of ``out`` where it is given) at the end."""
+    Sums are fp32 with one rounding to ``dtype`` (fp32, fp16 or bf16; that of ``out`` where it is given) at the end.
+    ``power_of_two``: the caller's word that every scale is one (``quantize_fp8`` makes no others), which large products are
+    faster for, the tensor cores then apply them; a scale that is not may make what it belongs to NaN."""
     if ta and not tb:
         raise ValueError("gemm_fp8: ta goes with tb")
     if not _native(a, a_scale, b, b_scale):
@@ -259,7 +262,7 @@ def gemm_fp8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: t
     sb_r, sb_c = b_scale.stride()
     _call(GEMM, out.get_device(), a.data_ptr(), lda, a_scale.data_ptr(), *((sa_c, sa_r) if ta else (sa_r, sa_c)), b.data_ptr(), ldb,
           b_scale.data_ptr(), *((sb_c, sb_r) if tb else (sb_r, sb_c)), out.data_ptr(), ldc, DTYPES[out.dtype], M, Nn, K, int(ta), int(tb),
-          nctas)
+          nctas, int(power_of_two))
     return out
 
 
