@@ -48,6 +48,16 @@ int sms_here() {
   return n;
 }
 
+// Columns of a tile of 256 rows where the tensor core applies the scales.  In 10 ns: a wave of 256 columns takes 35 a block of
+// 128 along K and 300 beside, and the last one 150 until its only accumulator is stored; a wave of 128 columns 22 and 136.
+// Measured (us, 256 / 128 columns): 8192 x 1792 x 4096 51.0 / 56.1, 8192 x 4096 x 4096 99.8 / 116.0, 8192 x 4096 x 1792 50.5 /
+// 59.2, 1792 x 4096 x 8192 51.0 / 61.0, 1024 x 4096 x 4096 16.8 / 19.2, 8192 x 512 x 8192 37.7 / 45.4, 2048 x 2048 x 2048
+// 14.1 / 13.2, 1024 x 14336 x 512 21.0 / 20.3.
+int pow2_columns(int64_t row_tiles, int64_t N, int64_t blocks, int64_t clusters) {
+  auto waves = [&](int bn) { return (row_tiles * ((N + bn - 1) / bn) + clusters - 1) / clusters; };
+  return waves(256) * (35 * blocks + 300) + 150 <= waves(128) * (22 * blocks + 136) ? 256 : 128;
+}
+
 int check_matrix(int64_t rows, int64_t cols, int64_t ldq, int dtype) {
   if (rows <= 0 || cols <= 0) return fail("rows and columns must be positive");
   if (!elem_size(dtype)) return fail("dtype must be fp32, fp16 or bf16");
@@ -178,7 +188,8 @@ static int gemm(void* stream, const void* A, int64_t lda, const void* sa, int64_
     // 10.6 / 8.1, 1001 x 1111 x 2050 13.0 / 11.0; 128 x 4096 x 1792 (14 blocks) 8.6 / 9.3 / 9.0.
     const int64_t nt = (N + 127) / 128, singles = (M + 127) / 128 * nt, blocks = (K + 127) / 128;
     const bool pair = M > 128 && sms > 1 && singles > sms;
-    const int64_t tiles = pair ? (M + 255) / 256 * nt : singles;
+    const int bn = pair && pow2 ? pow2_columns((M + 255) / 256, N, blocks, sms / 2) : 128;
+    const int64_t tiles = pair ? (M + 255) / 256 * ((N + bn - 1) / bn) : singles;
     int split = 1;
     while (!pair && split < 8 && tiles * split * 2 <= sms && split * 16 <= blocks) split *= 2;
     if (tiles > 0x3fffffffll) return fail("GEMM shape: too many tiles");
@@ -186,7 +197,7 @@ static int gemm(void* stream, const void* A, int64_t lda, const void* sa, int64_
     memset(&a, 0, sizeof(a));
     // K-major: boxes of 128 K x the CTA's rows; stored transposed: its columns x 128 K rows
     if (ta ? mthost::make_u8_map(&a.a, A, K, M, lda, 128) : mthost::make_u8_map(&a.a, A, M, K, lda, 128)) return -1;
-    if (tb ? mthost::make_u8_map(&a.b, B, K, N, ldb, 128, pair ? 64 : 128) : mthost::make_u8_map(&a.b, B, N, K, ldb, pair ? 64 : 128)) return -1;
+    if (tb ? mthost::make_u8_map(&a.b, B, K, N, ldb, 128, pair ? bn / 2 : 128) : mthost::make_u8_map(&a.b, B, N, K, ldb, pair ? bn / 2 : 128)) return -1;
     a.sa = (const float*)sa;
     a.sb = (const float*)sb;
     a.sa_m = sa_m;
@@ -203,7 +214,7 @@ static int gemm(void* stream, const void* A, int64_t lda, const void* sa, int64_
     a.timeout_ns = 4000000000ull;
     const int units = pair ? sms / 2 : sms, used = (int)(tiles < units ? tiles : units);
     const int grid = pair ? 2 * used : split > 1 ? split * (int)tiles : used;
-    if (launched(mt::launch_fp8_gemm(pair, pow2, split, ta != 0, tb != 0, a, grid, (cudaStream_t)stream), "fp8 gemm"))
+    if (launched(mt::launch_fp8_gemm(bn, pair, pow2, split, ta != 0, tb != 0, a, grid, (cudaStream_t)stream), "fp8 gemm"))
       return -1;
     mthost::stat_add(mthost::ST_GEMM, (uint64_t)(2.0 * M * N * K));
     return 0;

@@ -58,10 +58,10 @@ struct Fp8GemmArgs {
   int32_t vec_out;                  // rows of C start on 16-byte boundaries
   uint64_t timeout_ns;
 };
-// Tiles of 128 columns.  pair: 256 rows each, on CTA pairs (nctas even).  Else 128 rows each; split (1, 2, 4 or 8): the
+// bn: columns of a tile, 128, or 256 with pair and pow2.  pair: 256 rows each, on CTA pairs (nctas even).  Else 128 rows each; split (1, 2, 4 or 8): the
 // CTAs that share a tile's blocks along K, at most as many as there are blocks; nctas = split * tiles if it is not 1.
 // pow2: all scales are powers of two (looked at with pair only).
-cudaError_t launch_fp8_gemm(bool pair, bool pow2, int split, bool ta, bool tb, const Fp8GemmArgs& a, int nctas, cudaStream_t s);
+cudaError_t launch_fp8_gemm(int bn, bool pair, bool pow2, int split, bool ta, bool tb, const Fp8GemmArgs& a, int nctas, cudaStream_t s);
 int fp8_gemm_error();   // 1 after a wait of the kernel expired (synchronises), -1 on a CUDA error
 
 }  // namespace mt

@@ -59,9 +59,9 @@ template <int BN, bool PAIR, bool POW2 = false>
 struct Shape {
   static constexpr int BNC = PAIR ? BN / 2 : BN;          // rows of B staged by a CTA
   static constexpr uint32_t B_BYTES = BNC * BK;
-  static constexpr int STAGES = PAIR ? 7 : 5;
-  static constexpr uint32_t SF_BYTES = 1024;              // POW2: scale bytes of a stage, A's rows and B's
-  static constexpr int ACC = POW2 ? 2 : TMEM_COLS / BN;   // accumulators (POW2: the columns behind them hold scales)
+  static constexpr int STAGES = PAIR && BN == 128 ? 7 : 5;
+  static constexpr uint32_t SF_BYTES = 512 * (1 + BN / 128);   // POW2: scale bytes of a stage, A's rows and B's
+  static constexpr int ACC = POW2 ? 256 / BN : TMEM_COLS / BN;   // accumulators (POW2: the columns behind them hold scales)
   static constexpr uint32_t OPERANDS = STAGES * (A_BYTES + B_BYTES);
   static constexpr uint32_t RING = POW2 ? STAGES * SF_BYTES : kScaleSlots * 2 * BM * 4, STAGING = kSumWarps * 32 * kPitch;
   static constexpr uint32_t SMEM = 1024 + OPERANDS + RING + STAGING + 256;
@@ -195,7 +195,7 @@ __device__ __forceinline__ uint32_t scale_byte4(float s) {
 template <int BN, bool PAIR, bool POW2, bool TA, bool TB>
 __global__ void __launch_bounds__(kThreads, 1) gemm_fp8_kernel(const __grid_constant__ Fp8GemmArgs a) {
   static_assert(PAIR || !POW2, "the tensor core applies scales on pairs");
-  static_assert(!POW2 || Shape<BN, PAIR, POW2>::ACC * BN + Shape<BN, PAIR, POW2>::STAGES * 8 <= TMEM_COLS, "columns of TMEM");
+  static_assert(!POW2 || Shape<BN, PAIR, POW2>::ACC * BN + Shape<BN, PAIR, POW2>::STAGES * 16 <= TMEM_COLS, "columns of TMEM");
   using S = Shape<BN, PAIR, POW2>;
   constexpr int STAGES = S::STAGES, ACC = S::ACC, BNC = S::BNC, CW = BN / 2;   // CW: columns of a sum thread
   constexpr uint32_t B_BYTES = S::B_BYTES;
@@ -328,10 +328,11 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_fp8_kernel(const __grid_cons
                                            : make_smem_desc_mn_sw64(sB + s * B_BYTES);
           if (elect_one()) {
             if constexpr (POW2) {
-              const uint32_t sfa = tmem_base + ACC * BN + s * 8, sfb = sfa + 4;
+              const uint32_t sfa = tmem_base + ACC * BN + s * 16, sfb = sfa + 4;
               const uint8_t* sf = (const uint8_t*)sScale + s * S::SF_BYTES;
               tmem_cp_sf_pair(sfa, make_smem_desc_sf(sf));
               tmem_cp_sf_pair(sfb, make_smem_desc_sf(sf + 512));
+              if (BN > 128) tmem_cp_sf_pair(sfb + 4, make_smem_desc_sf(sf + 1024));
 #pragma unroll
               for (int k = 0; k < 4; ++k)
                 umma_mxfp8_pair(tmem_base + b * BN, da + k * step_a, db + k * step_b, make_idesc_mxfp8(kRows, BN, k, k) | trans, sfa, sfb,
@@ -399,9 +400,10 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_fp8_kernel(const __grid_cons
             if constexpr (POW2) {
               // byte (r % 32) * 16 + (r / 32) * 4 + k of an atom is row r's scale of the k-th 32 elements
               uint4* sf = (uint4*)((uint8_t*)sScale + s * S::SF_BYTES) + lane;
-              const uint32_t eb = scale_byte4(vb[j][0]);
+              const uint32_t eb = scale_byte4(vb[j][0]), eb1 = scale_byte4(vb[j][1]);
               sf[0] = make_uint4(scale_byte4(va[j][0]), scale_byte4(va[j][1]), scale_byte4(va[j][2]), scale_byte4(va[j][3]));
               sf[32] = make_uint4(eb, eb, eb, eb);
+              if (BN > 128) sf[64] = make_uint4(eb1, eb1, eb1, eb1);
               fence_proxy_async_smem();
             } else {
               float* f = sScale + ((pos + kb + 2 * j) & (kScaleSlots - 1)) * (2 * BM) + lane;
@@ -557,9 +559,10 @@ cudaError_t go_form(bool ta, bool tb, const Fp8GemmArgs& a, int cluster, int nct
 
 }  // namespace fp8g
 
-cudaError_t launch_fp8_gemm(bool pair, bool pow2, int split, bool ta, bool tb, const Fp8GemmArgs& a, int nctas, cudaStream_t s) {
-  if ((ta && !tb) || split < 1 || (pair && split > 1)) return cudaErrorInvalidValue;
+cudaError_t launch_fp8_gemm(int bn, bool pair, bool pow2, int split, bool ta, bool tb, const Fp8GemmArgs& a, int nctas, cudaStream_t s) {
+  if ((ta && !tb) || split < 1 || (pair && split > 1) || (bn != 128 && !(bn == 256 && pair && pow2))) return cudaErrorInvalidValue;
   count_launch();
+  if (bn == 256) return fp8g::go_form<256, true, true>(ta, tb, a, 2, nctas, s);
   if (pair) return pow2 ? fp8g::go_form<128, true, true>(ta, tb, a, 2, nctas, s) : fp8g::go_form<128, true, false>(ta, tb, a, 2, nctas, s);
   return fp8g::go_form<128, false, false>(ta, tb, a, split, nctas, s);
 }

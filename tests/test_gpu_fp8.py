@@ -130,7 +130,7 @@ def test_product_against_64_bits(size, form):
 
 
 @pytest.mark.parametrize("form", ["fwd", "dgrad", "wgrad"])
-@pytest.mark.parametrize("size", [(64, 100, 300), (2050, 1800, 260), (1500, 2301, 129), (2304, 2048, 1111), (300, 16384, 2050), (5000, 1000, 7)])
+@pytest.mark.parametrize("size", [(64, 100, 300), (2050, 1800, 260), (1500, 2301, 129), (2304, 2048, 1111), (300, 16384, 2050), (5000, 1000, 7), (1030, 4100, 4100), (8200, 520, 2100)])
 def test_product_with_scales_that_are_powers_of_two(size, form):
     a, b, *_ = operands(form, *size, spread=6.0)
     for _, s in (a, b):
