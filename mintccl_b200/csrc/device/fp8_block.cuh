@@ -278,31 +278,52 @@ __device__ __forceinline__ void restore16(const u128& w, float scale, float* f) 
 }
 
 // Where a thread of the row-block kernels works: eight lanes share a block of 128, 16 elements each, and a CTA of 256
-// threads has 32 blocks an item: of 32 rows where there are that many (their scales are neighbours in memory), else 32
-// blocks of one row.  Items are counted in 32 bits: a 64-bit division costs as much as a block.
-struct RowSpan {
-  int64_t row;
-  uint32_t kb;
-  bool live;
+// threads has 32 groups of U neighbouring blocks: of 32 rows where there are that many (their scales are neighbours in
+// memory), else of one row.  The grid has a column of CTAs for each 32 rows (or row) where it may be that high, else CTAs
+// find their place by a division; 64-bit divisions and one block a thread cost as much as the work on the block.
+struct RowGrid {
+  int64_t rows, cols;
+  uint32_t across;      // CTAs across a row
+  bool flat;            // one row of CTAs
 };
-__host__ __device__ __forceinline__ int64_t row_items(int64_t rows, int64_t nkb) {
-  return rows >= 32 ? (rows + 31) / 32 * nkb : rows * ((nkb + 31) / 32);
+template <int U>
+__host__ inline cudaError_t row_grid(int64_t rows, int64_t cols, RowGrid* g, dim3* grid) {
+  const int64_t groups = (cols + 128 * U - 1) / (128 * U), across = rows >= 32 ? groups : (groups + 31) / 32,
+                down = rows >= 32 ? (rows + 31) / 32 : rows;
+  if (across * down >= 0x7fffffffll) return cudaErrorInvalidValue;
+  *g = {rows, cols, (uint32_t)across, down > 65535};
+  *grid = g->flat ? dim3((unsigned)(across * down)) : dim3((unsigned)across, (unsigned)down);
+  return cudaSuccess;
 }
-__device__ __forceinline__ RowSpan row_span(uint32_t item, int g, int64_t rows, uint32_t nkb) {
-  RowSpan r;
-  if (rows >= 32) {
-    const uint32_t rt = item / nkb;
-    r.kb = item - rt * nkb;
-    r.row = (int64_t)rt * 32 + g;
-    r.live = r.row < rows;
-  } else {
-    const uint32_t chunks = (nkb + 31) / 32, row = item / chunks;
-    r.row = row;
-    r.kb = (item - row * chunks) * 32 + g;
-    r.live = r.row < rows && r.kb < nkb;
+template <int U>
+struct Place {
+  int64_t row, c0;      // the lane's first span; the others are 128 elements on
+  uint32_t kb;          // its block
+  int64_t left;         // elements of the row from that block on, 0 if there is no such row
+  __device__ __forceinline__ explicit Place(const RowGrid& g) {
+    const int gr = threadIdx.x >> 3;
+    uint32_t down = blockIdx.y, at = blockIdx.x;
+    if (g.flat) {
+      down = blockIdx.x / g.across;
+      at = blockIdx.x - down * g.across;
+    }
+    if (g.rows >= 32) {
+      row = (int64_t)down * 32 + gr;
+      kb = at * U;
+    } else {
+      row = down;
+      kb = (at * 32 + gr) * U;
+    }
+    const int64_t b0 = (int64_t)kb * 128;
+    c0 = b0 + (threadIdx.x & 7) * 16;
+    left = row < g.rows ? g.cols - b0 : 0;
   }
-  return r;
-}
+  // elements of span u that exist, and whether its block has any
+  __device__ __forceinline__ int n(int u) const {
+    return (int)min((int64_t)16, max((int64_t)0, left - (128 * u + (int)(threadIdx.x & 7) * 16)));
+  }
+  __device__ __forceinline__ bool live(int u) const { return left > 128 * u; }
+};
 
 // fp32 bits of the largest finite magnitudes of the row blocks that this lane's spans are parts of, all lanes of the warp
 // together; true if something in them was not finite.

@@ -49,126 +49,135 @@ __device__ __forceinline__ float silu_of(float x) {
   else return (0.25f * x) * rcp_fast(quarter_y(x));
 }
 
-// Where this thread works, and how many of its 16 elements exist.
-struct Place {
-  RowSpan at;
-  int64_t c0;
-  int n;
-  __device__ __forceinline__ Place(const Fp8ActArgs& a, uint32_t nkb) {
-    at = row_span(blockIdx.x, threadIdx.x >> 3, a.rows, nkb);
-    c0 = (int64_t)at.kb * 128 + (threadIdx.x & 7) * 16;
-    n = at.live ? (int)min((int64_t)16, max((int64_t)0, a.cols - c0)) : 0;
-  }
-};
-
-// 8192 x 4096 bf16: forward 35.5 us (4.7 TB/s), gated 49 (5.4), backward 34 (5.0), gated 54 (4.9); a copy runs at 6.0.  About 22
-// instructions an element are what is in the way: two spans a thread (34.6 forward, 58 - 69 the others) and more or fewer
-// CTAs than these an SM were slower.
-template <class T, int VEC, bool GATED>
-__global__ void __launch_bounds__(kThreads, 4) fp8_act_fwd_kernel(Fp8ActArgs a, uint32_t nkb) {
+// 8192 x 4096 bf16, us: forward 29.7 (5.7 TB/s), gated 48 (5.6), backward 29.6 (5.7), gated 53 (5.1); a copy runs at 6.0.  What is
+// in the way is some 18 instructions an element.  U: blocks a thread has in flight; with one the ungated forms took 36 and 34,
+// with two the gated ones 53 and 62.
+template <class T, int VEC, bool GATED, int U>
+__global__ void __launch_bounds__(kThreads, 4) fp8_act_fwd_kernel(Fp8ActArgs a, RowGrid grid) {
   using E = typename T::elem;
   using W = WarpSpans<T, VEC>;
   constexpr int kE = (int)sizeof(E);
   constexpr bool kExact = kE == 4;
   __shared__ __align__(16) uint8_t stages[8][W::kStage];
   uint8_t* stage = stages[threadIdx.x >> 5];
+  const Place<U> p(grid);
   const bool first = (threadIdx.x & 7) == 0;
-  const Place p(a, nkb);
-  const RowSpan& at = p.at;
-  Span16<T, VEC> h, g;
-  W::load(h, (const uint8_t*)a.h + (at.row * a.ldh + p.c0) * kE, p.n, stage);
-  if (GATED) W::load(g, (const uint8_t*)a.u + (at.row * a.ldu + p.c0) * kE, p.n, stage);
-  const bool put = at.live && p.c0 < a.ldq;
-  float f[16], y[16];
-  uint32_t e;
-  h.get(f);
+  const uint8_t* hp = (const uint8_t*)a.h + (p.row * a.ldh + p.c0) * kE;
+  const uint8_t* gp = GATED ? (const uint8_t*)a.u + (p.row * a.ldu + p.c0) * kE : nullptr;
+  Span16<T, VEC> h[U], g[U];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) y[i] = silu_of<kExact>(f[i]);
-  uint4 q = encode_row16(h, f, &e);
-  if (put) *(uint4*)(a.kh.data + at.row * a.ldq + p.c0) = q;
-  if (at.live && first) a.kh.scale[at.row * a.kh.s_row + at.kb * a.kh.s_col] = fp8_scale(e);
-  if (GATED) {
-    g.get(f);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) y[i] *= f[i];
-    q = encode_row16(g, f, &e);
-    if (put) *(uint4*)(a.ku.data + at.row * a.ldq + p.c0) = q;
-    if (at.live && first) a.ku.scale[at.row * a.ku.s_row + at.kb * a.ku.s_col] = fp8_scale(e);
+  for (int u = 0; u < U; ++u) {
+    W::load(h[u], hp + 128 * u * kE, p.n(u), stage);
+    if (GATED) W::load(g[u], gp + 128 * u * kE, p.n(u), stage);
   }
-  h.set(y);
-  W::store(h, (uint8_t*)a.y + (at.row * a.ldy + p.c0) * kE, p.n, stage);
+  const int64_t at = p.row * a.ldq + p.c0;
+  uint8_t* yp = (uint8_t*)a.y + (p.row * a.ldy + p.c0) * kE;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int n = p.n(u);
+    float f[16], y[16];
+    uint32_t e;
+    h[u].get(f);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) y[i] = silu_of<kExact>(f[i]);
+    uint4 q = encode_row16(h[u], f, &e);
+    if (n > 0) *(uint4*)(a.kh.data + at + 128 * u) = q;
+    if (first && p.live(u)) a.kh.scale[p.row * a.kh.s_row + (p.kb + u) * a.kh.s_col] = fp8_scale(e);
+    if (GATED) {
+      g[u].get(f);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) y[i] *= f[i];
+      q = encode_row16(g[u], f, &e);
+      if (n > 0) *(uint4*)(a.ku.data + at + 128 * u) = q;
+      if (first && p.live(u)) a.ku.scale[p.row * a.ku.s_row + (p.kb + u) * a.ku.s_col] = fp8_scale(e);
+    }
+    h[u].set(y);
+    W::store(h[u], yp + 128 * u * kE, n, stage);
+  }
 }
 
-template <class T, int VEC, bool GATED>
-__global__ void __launch_bounds__(kThreads) fp8_act_bwd_kernel(Fp8ActArgs a, uint32_t nkb) {
+template <class T, int VEC, bool GATED, int U>
+__global__ void __launch_bounds__(kThreads) fp8_act_bwd_kernel(Fp8ActArgs a, RowGrid grid) {
   using E = typename T::elem;
   using W = WarpSpans<T, VEC>;
   constexpr int kE = (int)sizeof(E);
   constexpr bool kExact = kE == 4;
   __shared__ __align__(16) uint8_t stages[8][W::kStage];
   uint8_t* stage = stages[threadIdx.x >> 5];
-  const Place p(a, nkb);
-  const RowSpan& at = p.at;
-  if (VEC > 0 && p.n <= 0) return;   // by elements the warp works as one
-  u128 hq = {0, 0}, gq = {0, 0};
-  float hs = 0.f, gs = 0.f;
-  if (VEC > 0 || p.n > 0) {
-    hq = load128_stream(a.kh.data + at.row * a.ldq + p.c0);
-    hs = __ldg(a.kh.scale + at.row * a.kh.s_row + at.kb * a.kh.s_col);
-    if (GATED) {
-      gq = load128_stream(a.ku.data + at.row * a.ldq + p.c0);
-      gs = __ldg(a.ku.scale + at.row * a.ku.s_row + at.kb * a.ku.s_col);
-    }
-  }
-  Span16<T, VEC> d;
-  W::load(d, (const uint8_t*)a.dy + (at.row * a.lddy + p.c0) * kE, p.n, stage);
-  float h[16], g[16], f[16], act[16];
-  restore16<F32>(hq, hs, h);
-  if (GATED) restore16<F32>(gq, gs, g);
-  d.get(f);
+  const Place<U> p(grid);
+  if (VEC > 0 && p.n(0) <= 0) return;   // by elements the warp works as one
+  const int64_t at = p.row * a.ldq + p.c0;
+  const uint8_t* dp = (const uint8_t*)a.dy + (p.row * a.lddy + p.c0) * kE;
+  u128 hq[U], gq[U];
+  float hs[U], gs[U];
+  Span16<T, VEC> d[U];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    // slope = s (1 + x (1 - s))
-    const float x = h[i], s = sigmoid_of<kExact>(x), slope = __fmaf_rn(s, __fmaf_rn(-s, x, x), s), y = x * s;
-    if (GATED) {
-      act[i] = y * g[i];
-      h[i] = f[i] * g[i] * slope;
-      g[i] = f[i] * y;
-    } else {
-      act[i] = y;
-      h[i] = f[i] * slope;
+  for (int u = 0; u < U; ++u) {
+    hq[u] = gq[u] = {0, 0};
+    hs[u] = gs[u] = 0.f;
+    if (p.n(u) > 0) {
+      hq[u] = load128_stream(a.kh.data + at + 128 * u);
+      hs[u] = __ldg(a.kh.scale + p.row * a.kh.s_row + (p.kb + u) * a.kh.s_col);
+      if (GATED) {
+        gq[u] = load128_stream(a.ku.data + at + 128 * u);
+        gs[u] = __ldg(a.ku.scale + p.row * a.ku.s_row + (p.kb + u) * a.ku.s_col);
+      }
     }
+    W::load(d[u], dp + 128 * u * kE, p.n(u), stage);
   }
-  d.set(h);
-  W::store(d, (uint8_t*)a.dh + (at.row * a.lddh + p.c0) * kE, p.n, stage);
-  if (GATED) {
-    d.set(g);
-    W::store(d, (uint8_t*)a.du + (at.row * a.lddu + p.c0) * kE, p.n, stage);
-  }
-  if (a.y) {
-    d.set(act);
-    W::store(d, (uint8_t*)a.y + (at.row * a.ldy + p.c0) * kE, p.n, stage);
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int n = p.n(u);
+    if (VEC > 0 && n <= 0) break;
+    float h[16], g[16], f[16], act[16];
+    restore16<F32>(hq[u], hs[u], h);
+    if (GATED) restore16<F32>(gq[u], gs[u], g);
+    d[u].get(f);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      // slope = s (1 + x (1 - s))
+      const float x = h[i], s = sigmoid_of<kExact>(x), slope = __fmaf_rn(s, __fmaf_rn(-s, x, x), s), y = x * s;
+      if (GATED) {
+        act[i] = y * g[i];
+        h[i] = f[i] * g[i] * slope;
+        g[i] = f[i] * y;
+      } else {
+        act[i] = y;
+        h[i] = f[i] * slope;
+      }
+    }
+    d[u].set(h);
+    W::store(d[u], (uint8_t*)a.dh + (p.row * a.lddh + p.c0 + 128 * u) * kE, n, stage);
+    if (GATED) {
+      d[u].set(g);
+      W::store(d[u], (uint8_t*)a.du + (p.row * a.lddu + p.c0 + 128 * u) * kE, n, stage);
+    }
+    if (a.y) {
+      d[u].set(act);
+      W::store(d[u], (uint8_t*)a.y + (p.row * a.ldy + p.c0 + 128 * u) * kE, n, stage);
+    }
   }
 }
 
-template <class T, int VEC>
+template <class T, int VEC, bool GATED>
 cudaError_t act_go(const Fp8ActArgs& a, bool forward, cudaStream_t s) {
-  const int64_t nkb = (a.cols + 127) / 128, items = row_items(a.rows, nkb);
-  const bool gated = forward ? a.u != nullptr : a.ku.data != nullptr;
-  if (items >= 0x7fffffffll) return cudaErrorInvalidValue;
-  auto go = [&](auto kernel) { kernel<<<(unsigned)items, kThreads, 0, s>>>(a, (uint32_t)nkb); };
-  if (forward) {
-    if (gated) go(fp8_act_fwd_kernel<T, VEC, true>);
-    else go(fp8_act_fwd_kernel<T, VEC, false>);
-  } else {
-    if (gated) go(fp8_act_bwd_kernel<T, VEC, true>);
-    else go(fp8_act_bwd_kernel<T, VEC, false>);
-  }
+  // spans a thread: two pay where they fit the registers of enough threads
+  constexpr int U = GATED || VEC == 0 ? 1 : 2;
+  RowGrid g;
+  dim3 grid;
+  if (cudaError_t e = row_grid<U>(a.rows, a.cols, &g, &grid); e != cudaSuccess) return e;
+  if (forward) fp8_act_fwd_kernel<T, VEC, GATED, U><<<grid, kThreads, 0, s>>>(a, g);
+  else fp8_act_bwd_kernel<T, VEC, GATED, U><<<grid, kThreads, 0, s>>>(a, g);
   return cudaGetLastError();
+}
+template <class T, int VEC>
+cudaError_t act_gated(const Fp8ActArgs& a, bool forward, cudaStream_t s) {
+  const bool gated = forward ? a.u != nullptr : a.ku.data != nullptr;
+  return gated ? act_go<T, VEC, true>(a, forward, s) : act_go<T, VEC, false>(a, forward, s);
 }
 template <class T>
 cudaError_t act_vec(const Fp8ActArgs& a, bool forward, cudaStream_t s) {
-  return a.vec == 2 ? act_go<T, 2>(a, forward, s) : a.vec == 1 ? act_go<T, 1>(a, forward, s) : act_go<T, 0>(a, forward, s);
+  return a.vec == 2 ? act_gated<T, 2>(a, forward, s) : a.vec == 1 ? act_gated<T, 1>(a, forward, s) : act_gated<T, 0>(a, forward, s);
 }
 cudaError_t act_any(int dtype, const Fp8ActArgs& a, bool forward, cudaStream_t s) {
   count_launch();

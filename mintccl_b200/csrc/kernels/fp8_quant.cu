@@ -13,43 +13,38 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// ---- row blocks: eight lanes a block, U blocks of every lane group in flight
+// ---- row blocks: eight lanes a block, U blocks of every lane group in flight.  8192 x 4096 bf16 takes 16.4 us (6.1 TB/s).
 template <class T, int VEC, int U>
-__global__ void __launch_bounds__(kThreads) fp8_row_kernel(Fp8QuantArgs a, uint32_t nkb, uint32_t items) {
+__global__ void __launch_bounds__(kThreads) fp8_row_kernel(Fp8QuantArgs a, RowGrid grid) {
   constexpr int kE = (int)sizeof(typename T::elem);
   using W = WarpSpans<T, VEC>;
   __shared__ __align__(16) uint8_t stage[8][W::kStage];
-  const int g = threadIdx.x >> 3, l = threadIdx.x & 7;
+  const Place<U> p(grid);
+  const uint8_t* x = (const uint8_t*)a.x + (p.row * a.ldx + p.c0) * kE;
   Span16<T, VEC> in[U];
-  RowSpan at[U];
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const uint32_t item = blockIdx.x * U + u;
-    at[u] = row_span(min(item, items - 1), g, a.rows, nkb);
-    at[u].live = at[u].live && item < items;
-    const int64_t c0 = (int64_t)at[u].kb * 128 + l * 16;
-    const int n = at[u].live ? (int)min((int64_t)16, max((int64_t)0, a.cols - c0)) : 0;
-    W::load(in[u], (const uint8_t*)a.x + (at[u].row * a.ldx + c0) * kE, n, stage[threadIdx.x >> 5]);
-  }
+  for (int u = 0; u < U; ++u) W::load(in[u], x + 128 * u * kE, p.n(u), stage[threadIdx.x >> 5]);
   uint32_t top[U];
   const bool special = row_tops<T, VEC, U>(in, top);
+  uint8_t* data = a.row.data + p.row * a.ldq + p.c0;
+  float* scale = a.row.scale + p.row * a.row.s_row + p.kb * a.row.s_col;
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     float f[16];
     in[u].get(f);
-    const uint32_t e = fp8_scale_exp(top[u]);
     only_finite16(f, special);
+    const uint32_t e = fp8_scale_exp(top[u]);
     const uint4 q = e4m3_16(f, fp8_inverse(e));
-    if (!at[u].live) continue;
-    const int64_t c0 = (int64_t)at[u].kb * 128 + l * 16;
-    if (c0 < a.ldq) *(uint4*)(a.row.data + at[u].row * a.ldq + c0) = q;   // the padding of a row is zeros
-    if (l == 0) a.row.scale[at[u].row * a.row.s_row + at[u].kb * a.row.s_col] = fp8_scale(e);
+    if (p.n(u) > 0) *(uint4*)(data + 128 * u) = q;   // a row's padding to 16 bytes is zeros
+    if ((threadIdx.x & 7) == 0 && p.live(u)) scale[u * a.row.s_col] = fp8_scale(e);
   }
 }
 
 // ---- any of the three from one read: a CTA holds a tile of 128 x 128 in registers, a thread 4 rows (32 apart) of 16
 // adjacent columns.  Largest magnitudes are taken on the bit patterns, two to a word; tiles with values that are not finite
-// look at them again.
+// look at them again.  8192 x 4096 bf16, us: tiles 17.3 (5.8 TB/s), column blocks 19.3, row blocks and tiles from one read 32 (4.2),
+// row and column blocks 35 (3.8; the two by themselves 36, with the input read twice): the second encoding of the same
+// registers is what these wait for, 128 of them a thread leave two CTAs an SM.
 template <class T, int VEC, bool ROW, bool COL, bool TILE>
 __global__ void __launch_bounds__(kThreads, sizeof(typename T::elem) == 2 && !ROW ? 3 : 2) fp8_tile_kernel(Fp8QuantArgs a, uint32_t nct) {
   constexpr int kE = (int)sizeof(typename T::elem);
@@ -181,9 +176,10 @@ cudaError_t quant_go(const Fp8QuantArgs& a, cudaStream_t s) {
     }
     return cudaGetLastError();
   }
-  const int64_t items = row_items(a.rows, nkb), grid = (items + 1) / 2;
-  if (items >= 0x7fffffffll) return cudaErrorInvalidValue;
-  fp8_row_kernel<T, VEC, 2><<<(unsigned)grid, kThreads, 0, s>>>(a, (uint32_t)nkb, (uint32_t)items);
+  RowGrid g;
+  dim3 grid;
+  if (cudaError_t e = row_grid<2>(a.rows, a.cols, &g, &grid); e != cudaSuccess) return e;
+  fp8_row_kernel<T, VEC, 2><<<grid, kThreads, 0, s>>>(a, g);
   return cudaGetLastError();
 }
 template <class T>
@@ -191,44 +187,55 @@ cudaError_t quant_vec(const Fp8QuantArgs& a, cudaStream_t s) {
   return a.vec == 2 ? quant_go<T, 2>(a, s) : a.vec == 1 ? quant_go<T, 1>(a, s) : quant_go<T, 0>(a, s);
 }
 
-// ---- decoding: 16 elements a thread
-template <class T, int VEC>
-__global__ void __launch_bounds__(kThreads) fp8_dequant_kernel(Fp8DequantArgs a, uint32_t nkb) {
+// ---- decoding: 8192 x 4096 bf16 takes 16.9 us (6.0 TB/s)
+template <class T, int VEC, int U>
+__global__ void __launch_bounds__(kThreads) fp8_dequant_kernel(Fp8DequantArgs a, RowGrid grid) {
   constexpr int kE = (int)sizeof(typename T::elem);
   using W = WarpSpans<T, VEC>;
   __shared__ __align__(16) uint8_t stage[8][W::kStage];
-  const int g = threadIdx.x >> 3, l = threadIdx.x & 7;
-  const RowSpan at = row_span(blockIdx.x, g, a.rows, nkb);
-  const int64_t c0 = (int64_t)at.kb * 128 + l * 16;
-  const int n = at.live ? (int)min((int64_t)16, max((int64_t)0, a.cols - c0)) : 0;
-  if (VEC > 0 && n <= 0) return;   // by elements the warp works as one
-  float f[16];
+  const Place<U> p(grid);
+  if (VEC > 0 && p.n(0) <= 0) return;   // by elements the warp works as one
+  const uint8_t* data = a.data + p.row * a.ldq + p.c0;
+  const float* sp = a.scale + (p.row >> a.rshift) * a.s_row;
+  uint8_t* out = (uint8_t*)a.out + (p.row * a.ldo + p.c0) * kE;
+  u128 w[U];
+  float sc[U];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) f[i] = 0.f;
-  if (VEC > 0 || n > 0) {
-    const u128 w = load128_stream(a.data + at.row * a.ldq + c0);
-    const float* sp = a.scale + (at.row >> a.rshift) * a.s_row;
-    if (a.cshift) {
-      restore16<T>(w, __ldg(sp + at.kb * a.s_col), f);
-    } else {
-      float sc[16];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) sc[i] = i < n ? __ldg(sp + (c0 + i) * a.s_col) : 0.f;
-      restore16<F32>(w, 1.f, f);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) f[i] = clamp_nan(f[i] * sc[i], MaxOf<T>::value);
+  for (int u = 0; u < U; ++u) {
+    w[u] = {0, 0};
+    sc[u] = 1.f;
+    if (p.n(u) > 0) {
+      w[u] = load128_stream(data + 128 * u);
+      if (a.cshift) sc[u] = __ldg(sp + (p.kb + u) * a.s_col);
     }
   }
-  Span16<T, VEC> o;
-  o.set(f);
-  W::store(o, (uint8_t*)a.out + (at.row * a.ldo + c0) * kE, n, stage[threadIdx.x >> 5]);
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int n = p.n(u);
+    if (VEC > 0 && n <= 0) break;
+    float f[16];
+    if (a.cshift) {
+      restore16<T>(w[u], sc[u], f);
+    } else {
+      float c[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) c[i] = i < n ? __ldg(sp + (p.c0 + 128 * u + i) * a.s_col) : 0.f;
+      restore16<F32>(w[u], 1.f, f);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) f[i] = clamp_nan(f[i] * c[i], MaxOf<T>::value);
+    }
+    Span16<T, VEC> o;
+    o.set(f);
+    W::store(o, out + 128 * u * kE, n, stage[threadIdx.x >> 5]);
+  }
 }
 
 template <class T, int VEC>
 cudaError_t dequant_go(const Fp8DequantArgs& a, cudaStream_t s) {
-  const int64_t nkb = (a.cols + 127) / 128, items = row_items(a.rows, nkb);
-  if (items >= 0x7fffffffll) return cudaErrorInvalidValue;
-  fp8_dequant_kernel<T, VEC><<<(unsigned)items, kThreads, 0, s>>>(a, (uint32_t)nkb);
+  RowGrid g;
+  dim3 grid;
+  if (cudaError_t e = row_grid<2>(a.rows, a.cols, &g, &grid); e != cudaSuccess) return e;
+  fp8_dequant_kernel<T, VEC, 2><<<grid, kThreads, 0, s>>>(a, g);
   return cudaGetLastError();
 }
 template <class T>

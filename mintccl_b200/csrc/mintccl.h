@@ -156,8 +156,8 @@ int mt_mxfp8_quantize(void* stream, int dtype, const void* x, void* data, void* 
 int mt_mxfp8_tile_scales(void* stream, const void* in, void* out, uint64_t rows, uint64_t kb);
 
 // ---- e4m3 with one fp32 scale per block of 128 (host/fp8_host.cu), on the current device -------------------------------
-// Payload rows are ldq bytes apart (a multiple of 16, at least cols; padding is written as zeros) and start on 16-byte
-// boundaries.  dtype: 0 fp32, 1 fp16, 2 bf16.  ld*: elements between rows.
+// Payload rows are ldq bytes apart (a multiple of 16, at least cols; padding up to the next 16 is written as zeros) and start on
+// 16-byte boundaries.  dtype: 0 fp32, 1 fp16, 2 bf16.  ld*: elements between rows.
 // Encodings of x [rows, cols]; any of the three may be null.  row_scale [ceil(cols / 128)][rows] (of blocks 1 x 128),
 // col_scale [ceil(rows / 128)][cols] (128 x 1), tile_scale [ceil(rows / 128)][ceil(cols / 128)].
 int mt_fp8_quantize(void* stream, int dtype, const void* x, int64_t ldx, int64_t rows, int64_t cols, int64_t ldq,
