@@ -1,6 +1,6 @@
 """Times the tcgen05 GEMM against cuBLAS (torch.matmul) on one GPU.
 
-    python mintccl_b200/benchmarks/gemm_bench.py [--shapes 8192x1792x4096,8192x4096x1792] [--iters 20]
+    python mintccl_b200/benchmarks/gemm_bench.py [--shapes 8192x1792x4096,8192x4096x1792] [--iters 20] [--mxfp8] [--fp8]
 
 Each shape is MxNxK for ``a[M, K] @ w[N, K].T``.  Device time from CUDA events after warm-up; operands and
 outputs of consecutive calls rotate through a pool larger than the L2.
@@ -23,6 +23,7 @@ def main() -> None:
     ap.add_argument("--iters", type=int, default=20)
     ap.add_argument("--nctas", type=int, default=0)
     ap.add_argument("--mxfp8", action="store_true", help="also time the block-scaled fp8 GEMM on each shape")
+    ap.add_argument("--fp8", action="store_true", help="also time the e4m3 GEMM with a scale per block of 128, of any value and powers of two")
     a = ap.parse_args()
     from mintccl_b200.ops.gemm import gemm
     for shape in a.shapes.split(","):
@@ -70,6 +71,23 @@ def main() -> None:
             ms = e0.elapsed_time(e1) / a.iters
             row["mxfp8_us"] = round(ms * 1e3, 1)
             row["mxfp8_tflops"] = round(row["flop"] / (ms * 1e-3) / 1e12, 1)
+        if a.fp8:
+            from mintccl_b200.ops import fp8
+            c8 = max(2, (300 << 20) // (M * K + N * K + M * N * 2) + 1)
+            qs = [(*fp8.quantize_fp8(As[i % copies]), *fp8.quantize_fp8(Ws[i % copies], "tile")) for i in range(c8)]
+            for name, pow2 in (("fp8", False), ("fp8_pow2", True)):
+                for i in range(5):
+                    fp8.gemm_fp8(*qs[i % c8], out=Os[i % copies], nctas=a.nctas, power_of_two=pow2)
+                torch.cuda.synchronize()
+                e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+                e0.record()
+                for i in range(a.iters):
+                    fp8.gemm_fp8(*qs[i % c8], out=Os[i % copies], nctas=a.nctas, power_of_two=pow2)
+                e1.record()
+                torch.cuda.synchronize()
+                ms = e0.elapsed_time(e1) / a.iters
+                row[name + "_us"] = round(ms * 1e3, 1)
+                row[name + "_tflops"] = round(row["flop"] / (ms * 1e-3) / 1e12, 1)
         print(json.dumps(row), flush=True)
 
 

@@ -1,1 +1,1 @@
-"""Collective operations (module-level API), fused GEMM+collective ops and the LL128 layout oracle."""
+"""Collective operations (module-level API), fused GEMM+collective ops, 8-bit formats and their products, and the LL128 layout oracle."""
