@@ -96,6 +96,12 @@ struct Span16 {
       for (int i = 0; i < kWords; ++i) v[i] = i < n ? __ldg(e + i) : 0u;
     }
   }
+  // What follows unpacks the words anew: without this the compiler keeps the fp32 values of an earlier use alive, at twice the
+  // registers of the words.
+  __device__ __forceinline__ void again() {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) asm volatile("" : "+r"(v[i]));
+  }
   __device__ __forceinline__ void clear(int n) {   // elements from the n-th on
 #pragma unroll
     for (int i = 0; i < kWords; ++i) {

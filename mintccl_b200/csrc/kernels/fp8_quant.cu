@@ -42,9 +42,9 @@ __global__ void __launch_bounds__(kThreads) fp8_row_kernel(Fp8QuantArgs a, RowGr
 
 // ---- any of the three from one read: a CTA holds a tile of 128 x 128 in registers, a thread 4 rows (32 apart) of 16
 // adjacent columns.  Largest magnitudes are taken on the bit patterns, two to a word; tiles with values that are not finite
-// look at them again.  8192 x 4096 bf16, us: tiles 17.3 (5.8 TB/s), column blocks 19.3, row blocks and tiles from one read 32 (4.2),
-// row and column blocks 35 (3.8; the two by themselves 36, with the input read twice): the second encoding of the same
-// registers is what these wait for, 128 of them a thread leave two CTAs an SM.
+// look at them again.  8192 x 4096 bf16, us: tiles 17.3 (5.8 TB/s), column blocks 18.9, row blocks and tiles from one read 29 (4.6),
+// row and column blocks 32 (4.2); one after the other these two take 35 and 36.5, with the input from the L2 the second time.
+// The 125 registers that two encodings of the same words take leave two CTAs an SM; three spill (50 - 60 us).
 template <class T, int VEC, bool ROW, bool COL, bool TILE>
 __global__ void __launch_bounds__(kThreads, sizeof(typename T::elem) == 2 && !ROW ? 3 : 2) fp8_tile_kernel(Fp8QuantArgs a, uint32_t nct) {
   constexpr int kE = (int)sizeof(typename T::elem);
@@ -58,26 +58,30 @@ __global__ void __launch_bounds__(kThreads, sizeof(typename T::elem) == 2 && !RO
   const uint32_t rt = blockIdx.x / nct, ct = blockIdx.x - rt * nct;
   const int64_t c0 = (int64_t)ct * 128 + l * 16;
   const int n = (int)min((int64_t)16, max((int64_t)0, a.cols - c0));
+  // rows of this thread that exist, of four; where the first is in a payload, and the distance to the next
+  const int64_t r0 = (int64_t)rt * 128 + g, q0 = r0 * a.ldq + c0, qstep = 32 * a.ldq;
+  const int live = (int)min((int64_t)4, max((int64_t)0, (a.rows - r0 + 31) >> 5));
+  const bool put = c0 < a.ldq;
   Span16<T, VEC> in[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t r = (int64_t)rt * 128 + i * 32 + g;
-    W::load(in[i], (const uint8_t*)a.x + (r * a.ldx + c0) * kE, r < a.rows ? n : 0, stage[warp]);
-  }
+  for (int i = 0; i < 4; ++i)
+    W::load(in[i], (const uint8_t*)a.x + ((r0 + i * 32) * a.ldx + c0) * kE, i < live ? n : 0, stage[warp]);
   if (ROW) {
     uint32_t top[4];
     const bool special = row_tops<T, VEC, 4>(in, top);
+    uint8_t* to = a.row.data + q0;
+    float* scale = a.row.scale + r0 * a.row.s_row + ct * a.row.s_col;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int64_t r = (int64_t)rt * 128 + i * 32 + g;
+    for (int i = 0; i < 4; ++i, to += qstep, scale += 32 * a.row.s_row) {
       float f[16];
+      in[i].again();
       in[i].get(f);
       only_finite16(f, special);
       const uint32_t e = fp8_scale_exp(top[i]);
       const uint4 q = e4m3_16(f, fp8_inverse(e));
-      if (r < a.rows) {
-        if (c0 < a.ldq) *(uint4*)(a.row.data + r * a.ldq + c0) = q;
-        if (l == 0) a.row.scale[r * a.row.s_row + ct * a.row.s_col] = fp8_scale(e);
+      if (i < live) {
+        if (put) *(uint4*)to = q;
+        if (l == 0) *scale = fp8_scale(e);
       }
     }
   }
@@ -116,14 +120,15 @@ __global__ void __launch_bounds__(kThreads, sizeof(typename T::elem) == 2 && !RO
     for (int w = 0; w < 8; ++w) t = max(t, s_tile[w]);
     const uint32_t e = fp8_scale_exp(t);
     const float inv = fp8_inverse(e);
+    uint8_t* to = a.tile.data + q0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int64_t r = (int64_t)rt * 128 + i * 32 + g;
+    for (int i = 0; i < 4; ++i, to += qstep) {
       float f[16];
+      in[i].again();
       in[i].get(f);
       only_finite16(f, special);
       const uint4 q = e4m3_16(f, inv);
-      if (r < a.rows && c0 < a.ldq) *(uint4*)(a.tile.data + r * a.ldq + c0) = q;
+      if (i < live && put) *(uint4*)to = q;
     }
     if (threadIdx.x == 0) a.tile.scale[rt * a.tile.s_row + ct * a.tile.s_col] = fp8_scale(e);
   }
@@ -144,15 +149,17 @@ __global__ void __launch_bounds__(kThreads, sizeof(typename T::elem) == 2 && !RO
     float inv[16];
 #pragma unroll
     for (int j = 0; j < 4; ++j) *(float4*)(inv + 4 * j) = *(const float4*)(s_inv + l * 16 + 4 * j);
+    uint8_t* to = a.col.data + q0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int64_t r = (int64_t)rt * 128 + i * 32 + g;
+    for (int i = 0; i < 4; ++i, to += qstep) {
       float f[16];
+      in[i].again();
       in[i].get(f);
       only_finite16(f, special);
 #pragma unroll
       for (int j = 0; j < 16; ++j) f[j] *= inv[j];
-      if (r < a.rows && c0 < a.ldq) *(uint4*)(a.col.data + r * a.ldq + c0) = e4m3_16(f, 1.f);
+      const uint4 q = e4m3_16(f, 1.f);
+      if (i < live && put) *(uint4*)to = q;
     }
   }
 }
