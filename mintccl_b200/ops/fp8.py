@@ -70,10 +70,6 @@ def _native(*ts: torch.Tensor) -> bool:
     return True
 
 
-def _cdiv(a: int, b: int) -> int:
-    return -(-a // b)
-
-
 def _up16(n: int) -> int:
     return (n + 15) & ~15
 
@@ -267,55 +263,48 @@ def gemm_fp8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: t
 
 
 # ---- the linear layer ----------------------------------------------------------------------------------------------
-def _areas(*sizes: int) -> Tuple[List[int], int]:
-    """Offsets of areas of these sizes in one buffer (allocating each by itself is most of a small layer's time), and its size."""
-    offs, at = [], 0
-    for n in sizes:
-        offs.append(at)
-        at += (n + 255) & ~255
-    return offs, at
-
-
-def _sizes(rows: int, cols: int, block: str) -> Tuple[int, int]:
-    r, c = _scale_shape(rows, cols, block)
-    return rows * _up16(cols), 4 * r * c
+def _room(nbytes: int) -> int:
+    """Areas of one buffer start 256 bytes apart: allocating each by itself is most of a small layer's time."""
+    return (nbytes + 255) & ~255
 
 
 class _LinearFp8(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, w_data, w_scale, keep):
         # keep: the weight has a gradient, which contracts over the tokens; what is kept of x for it are tiles, in 8 bits
-        (n, k), dev = w.shape, x.device
-        x2, ldx = _rows(x.reshape(-1, k))
-        t = x2.shape[0]
-        own = w_data is None
-        offs, size = _areas(*(_sizes(t, k, "tile") if keep else (0, 0)), *(_sizes(n, k, "tile") if own else (0, 0)))
-        kept = torch.empty(size, device=dev, dtype=torch.uint8) if size else None
+        n, k = w.shape
+        x2, ldx = _rows(x if x.dim() == 2 else x.reshape(-1, k))
+        t, pk, kb, own = x2.shape[0], (k + 15) & ~15, -(-k // BLOCK), w_data is None
+        # one buffer: x's tiles and their scales, w's tiles and theirs
+        xs = _room(t * pk) if keep else 0
+        wd = xs + (_room(4 * -(-t // BLOCK) * kb) if keep else 0)
+        ws = wd + (_room(n * pk) if own else 0)
+        size = ws + (4 * -(-n // BLOCK) * kb if own else 0)
+        kept = x2.new_empty(size, dtype=torch.uint8) if size else None
         base = kept.data_ptr() if size else 0
-        ctx.sizes = t, n, k, offs, size, x.dtype, w.dtype
+        ctx.sizes = t, n, k, xs, wd, ws, size, x.dtype, w.dtype
         ctx.save_for_backward(kept, w_data, w_scale)
-        y = torch.empty((*x.shape[:-1], n), device=dev, dtype=x.dtype)
+        y = x2.new_empty((t, n) if x.dim() == 2 else (*x.shape[:-1], n))
         if own:
-            w2, ldw = _rows(w.detach())
-            wq = w2.data_ptr(), ldw, base + offs[2], _up16(k), base + offs[3], -(-k // BLOCK), 1
+            w2, ldw = _rows(w)
+            wq = w2.data_ptr(), ldw, base + wd, pk, base + ws, kb, 1
         else:
             w2, pitch = _payload(w_data, "w_fp8")
             wq = 0, 0, w2.data_ptr(), pitch, w_scale.data_ptr(), *w_scale.stride()
         if t:
-            (data_at, scale_at), room = _areas(*_sizes(t, k, "row"))
-            tmp = torch.empty(room, device=dev, dtype=torch.uint8)
-            at = tmp.data_ptr()
-            _call(LINEAR_FORWARD, y.get_device(), DTYPES[x.dtype], x2.data_ptr(), ldx, t, k, DTYPES[w.dtype], wq[0], wq[1], n,
-                  at + data_at, at + scale_at, *((base + offs[0], base + offs[1]) if keep else (0, 0)), *wq[2:], y.data_ptr())
+            rows = x2.new_empty(_room(t * pk) + 4 * t * kb, dtype=torch.uint8)      # x's row blocks, for this product only
+            at = rows.data_ptr()
+            _call(LINEAR_FORWARD, y.get_device(), DTYPES[x.dtype], x2.data_ptr(), ldx, t, k, DTYPES[w.dtype], wq[0], wq[1], n, at,
+                  at + _room(t * pk), base if keep else 0, base + xs if keep else 0, *wq[2:], y.data_ptr())
         elif own:
-            _call(QUANTIZE, y.get_device(), DTYPES[w.dtype], wq[0], wq[1], n, k, wq[3], 0, 0, 0, 0, wq[2], wq[4])
+            _call(QUANTIZE, y.get_device(), DTYPES[w.dtype], wq[0], wq[1], n, k, pk, 0, 0, 0, 0, wq[2], wq[4])
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         kept, w_data, w_scale = ctx.saved_tensors
-        t, n, k, offs, size, x_dtype, w_dtype = ctx.sizes
+        t, n, k, xs, wd, ws, size, x_dtype, w_dtype = ctx.sizes
         want_x, want_w = ctx.needs_input_grad[:2]
         if not _native(dy):
             raise ValueError("the gradient must be a plain CUDA tensor, and nobody recording")
@@ -326,20 +315,23 @@ class _LinearFp8(torch.autograd.Function):
                 kept = kept.clone()
             base = kept.data_ptr()
         if w_data is None:
-            w2, wq = None, (base + offs[2], _up16(k), base + offs[3], -(-k // BLOCK), 1)
+            w2, wq = None, (base + wd, (k + 15) & ~15, base + ws, -(-k // BLOCK), 1)
         else:
             w2, pitch = _payload(w_data, "w_fp8")
             wq = w2.data_ptr(), pitch, w_scale.data_ptr(), *w_scale.stride()
-        dx = torch.empty((*dy.shape[:-1], k), device=dy.device, dtype=x_dtype) if want_x else None
-        dw = torch.empty((n, k), device=dy.device, dtype=w_dtype) if want_w else None
+        dx = dy.new_empty((*dy.shape[:-1], k), dtype=x_dtype) if want_x else None
+        dw = dy.new_empty((n, k), dtype=w_dtype) if want_w else None
         if t and (want_x or want_w):
-            dy2, ld = _rows(dy.reshape(-1, n))
-            (rd, rs, cd, cs), room = _areas(*(_sizes(t, n, "row") if want_x else (0, 0)), *(_sizes(t, n, "col") if want_w else (0, 0)))
-            tmp = torch.empty(room, device=dy.device, dtype=torch.uint8)
+            dy2, ld = _rows(dy if dy.dim() == 2 else dy.reshape(-1, n))
+            # dy's row blocks and their scales, its column blocks and theirs
+            pn = (n + 15) & ~15
+            rs = _room(t * pn) if want_x else 0
+            cd = rs + (_room(4 * t * -(-n // BLOCK)) if want_x else 0)
+            cs = cd + (_room(t * pn) if want_w else 0)
+            tmp = dy2.new_empty(cs + (4 * -(-t // BLOCK) * n if want_w else 0), dtype=torch.uint8)
             at = tmp.data_ptr()
-            _call(LINEAR_BACKWARD, dy.get_device(), DTYPES[x_dtype], dy2.data_ptr(), ld, t, n, k, at + rd, at + rs, *wq,
-                  dx.data_ptr() if want_x else 0, at + cd, at + cs, base + offs[0], base + offs[1], dw.data_ptr() if want_w else 0,
-                  DTYPES[w_dtype])
+            _call(LINEAR_BACKWARD, dy2.get_device(), DTYPES[x_dtype], dy2.data_ptr(), ld, t, n, k, at, at + rs, *wq,
+                  dx.data_ptr() if want_x else 0, at + cd, at + cs, base, base + xs, dw.data_ptr() if want_w else 0, DTYPES[w_dtype])
         elif want_w:
             dw.zero_()
         return dx, dw, None, None, None
