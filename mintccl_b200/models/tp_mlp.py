@@ -28,8 +28,8 @@ def _operand(t: torch.Tensor) -> torch.Tensor:
 class _MLPFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x_shard, w_up, w_down, mlp):
-        ctx.mlp = mlp
-        if mlp.checkpoint == "fp8":
+        ctx.mlp, ctx.checkpoint = mlp, mlp.checkpoint
+        if ctx.checkpoint == "fp8":
             # of [T, F/n] only h is kept, in 8 bits: 1.03 bytes an element instead of 4
             a, kept = silu8_forward(mlp.ag_gemm(x_shard, w_up))
             kept = kept.data, kept.scale
@@ -61,7 +61,7 @@ class _MLPFunction(torch.autograd.Function):
             x = x_shard.new_empty((n, *x_shard.shape))
             comm.allgather(x, inp=x_shard)
             x = x.view(T, -1)
-        if mlp.checkpoint == "fp8":
+        if ctx.checkpoint == "fp8":
             da = gemm_t(dy, w_down, tb=True)                 # [T, F/n] = dy @ w_down   (w_down: [H, F/n])
             dh, a = silu8_backward(Saved8(*kept, da.shape, da.dtype), da, act=True)
         else:

@@ -232,6 +232,51 @@ def test_mlp_of_two_ranks_with_its_activation_input_in_8_bits(between, monkeypat
                 torch.testing.assert_close(a, b, rtol=1e-4, atol=1e-4)     # fp32 sums of at most 20 terms
 
 
+@pytest.mark.parametrize("order", [("fp8", None), (None, "fp8")], ids=str)
+def test_mlp_whose_checkpoint_is_changed_between_the_passes(order, monkeypatch):
+    """The backward pass follows what its own forward pass has kept."""
+    import threading
+
+    import test_cpu_tp_mlp as two
+    from mintccl_b200.models import tp_mlp
+
+    class Gather(two.FakeGather):
+        def __call__(self, x, w):
+            return self.call_silu(x, w)[0]
+
+    monkeypatch.setattr(tp_mlp, "gemm_t", lambda a, b, ta=False, tb=False: (a.t() if ta else a) @ (b if tb else b.t()))
+    monkeypatch.setattr(tp_mlp, "gemm_dsilu", two.dsilu)
+    g = torch.Generator().manual_seed(5)
+    N, T, H, F = two.N, two.T, two.H, two.F
+    ups, downs = torch.randn(N, F, H, generator=g), torch.randn(N, H, F, generator=g)
+    xs, dys = torch.randn(T, H, generator=g), torch.randn(T, H, generator=g)
+    got, errors, per = {}, [], T // N
+
+    def rank(r, bus, change):
+        try:
+            m, rows = two.mlp_of(two.Comm(bus, r), ups[r], downs[r]), slice(r * per, (r + 1) * per)
+            m.checkpoint, m.ag_gemm = order[0], Gather(m.comm)
+            s = xs[rows].clone().requires_grad_(True)
+            y = m(s)
+            if change:
+                m.checkpoint = order[1]
+            got[r, change] = torch.autograd.grad(y, [s, m.w_up, m.w_down], dys[rows])
+        except Exception as e:
+            errors.append(e)
+            bus.bar.abort()
+
+    for change in (False, True):
+        bus = two.Bus()
+        threads = [threading.Thread(target=rank, args=(r, bus, change)) for r in range(N)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join(60)
+        assert not errors, errors
+    for r in range(N):
+        assert all(torch.equal(a, b) for a, b in zip(got[r, True], got[r, False]))
+
+
 def test_mlp_refuses_unknown_checkpoints():
     from mintccl_b200.models import tp_mlp
 
