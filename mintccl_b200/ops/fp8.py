@@ -221,7 +221,7 @@ def gemm_fp8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: t
     * ``tb``: ``a [M, K] @ b [K, N]``: the gradient of its input; ``a`` in row blocks, ``b`` in tiles;
     * ``ta`` and ``tb``: ``a[K, M].T @ b [K, N]``: the gradient of its weight; ``a`` in column blocks, ``b`` in tiles.
 
-    Sums are fp32 with one rounding to ``dtype`` (fp32, fp16 or bf16; that of ``out`` where it is given) at the end.
+    Sums are fp32, the product of two blocks' scales has to be in that range too, with one rounding to ``dtype`` (fp32, fp16 or bf16; that of ``out`` where it is given) at the end.
     ``power_of_two``: the caller's word that every scale is one (``quantize_fp8`` makes no others), which large products are
     faster for, the tensor cores then apply them; a scale that is not may make what it belongs to NaN."""
     if ta and not tb:
@@ -263,6 +263,12 @@ def gemm_fp8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: t
 
 
 # ---- the linear layer ----------------------------------------------------------------------------------------------
+def _check_encoded(data: torch.Tensor, scale: torch.Tensor, shape: Tuple[int, int], like: torch.Tensor) -> None:
+    if data.shape != shape or data.dtype not in _U8 or not _native(data, scale) or data.device != like.device:
+        raise ValueError("w_fp8 does not belong to w")
+    _check_scale(scale, _scale_shape(*shape, "tile"), data, "the scales of w_fp8")
+
+
 def _room(nbytes: int) -> int:
     """Areas of one buffer start 256 bytes apart: allocating each by itself is most of a small layer's time."""
     return (nbytes + 255) & ~255
@@ -310,6 +316,8 @@ class _LinearFp8(torch.autograd.Function):
             raise ValueError("the gradient must be a plain CUDA tensor, and nobody recording")
         base = 0
         if size:   # what a saved-tensor hook made of it
+            if kept.dtype != torch.uint8 or kept.numel() != size or kept.device != dy.device or not _native(kept):
+                raise ValueError("what was kept for the gradient came back as another tensor")
             kept = kept.contiguous()
             if kept.data_ptr() % 16:
                 kept = kept.clone()
@@ -317,6 +325,7 @@ class _LinearFp8(torch.autograd.Function):
         if w_data is None:
             w2, wq = None, (base + wd, (k + 15) & ~15, base + ws, -(-k // BLOCK), 1)
         else:
+            _check_encoded(w_data, w_scale, (n, k), dy)
             w2, pitch = _payload(w_data, "w_fp8")
             wq = w2.data_ptr(), pitch, w_scale.data_ptr(), *w_scale.stride()
         dx = dy.new_empty((*dy.shape[:-1], k), dtype=x_dtype) if want_x else None
@@ -356,7 +365,5 @@ def linear_fp8(x: torch.Tensor, w: torch.Tensor, w_fp8: Optional[Quantized] = No
         raise ValueError("x and w must be plain CUDA tensors, and nobody recording")
     data, scale = w_fp8 if w_fp8 is not None else (None, None)
     if data is not None:
-        if data.shape != w.shape or data.dtype not in _U8 or not _native(data, scale) or data.device != w.device:
-            raise ValueError("w_fp8 does not belong to w")
-        _check_scale(scale, _scale_shape(*w.shape, "tile"), data, "the scales of w_fp8")
+        _check_encoded(data, scale, tuple(w.shape), w)
     return _LinearFp8.apply(x, w, data, scale, torch.is_grad_enabled() and w.requires_grad)

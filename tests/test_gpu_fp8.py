@@ -352,6 +352,23 @@ def test_saved_tensor_hooks_may_change_the_layout():
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("unpack", [lambda t: t.cpu(), lambda t: t[:-1] if t.dim() == 1 else t[:, :-1], lambda t: t.float()],
+                         ids=["host", "shorter", "type"])
+@pytest.mark.parametrize("given", [False, True], ids=["weight", "encoded_weight"])
+def test_saved_tensors_that_come_back_wrong_are_refused(given, unpack):
+    x = torch.randn(130, 300, device="cuda", requires_grad=True)
+    w = torch.randn(70, 300, device="cuda", requires_grad=not given)
+    encoded = fp8.quantize_fp8(w, "tile") if given else None      # then it is all that is kept
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+        y = fp8.linear_fp8(x, w, encoded)
+    with pytest.raises(ValueError):
+        y.sum().backward()
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+        y = c8.silu8(x)
+    with pytest.raises((ValueError, RuntimeError)):
+        y.sum().backward()
+
+
 def test_training_step_in_a_graph():
     """Forward and backward captured once and replayed on other data give what the eager step gives."""
     g = torch.Generator(device="cuda").manual_seed(5)
