@@ -23,15 +23,40 @@ __device__ __forceinline__ uint32_t fp8_scale_exp(uint32_t amax) {
 __device__ __forceinline__ float fp8_scale(uint32_t e) { return __uint_as_float(e << 23); }
 __device__ __forceinline__ float fp8_inverse(uint32_t e) { return __uint_as_float((254u - e) << 23); }   // e <= 247
 
+// Two fp32 operations in one instruction, each rounded as by itself.
+struct F2 {
+  uint64_t v;
+  __device__ __forceinline__ F2(float lo, float hi) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi)); }
+  __device__ __forceinline__ explicit F2(float both) : F2(both, both) {}
+  __device__ __forceinline__ void get(float& lo, float& hi) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+};
+__device__ __forceinline__ F2 operator*(F2 a, F2 b) {
+  asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(a.v) : "l"(b.v));
+  return a;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  asm("fma.rn.f32x2 %0, %0, %1, %2;" : "+l"(a.v) : "l"(b.v), "l"(c.v));
+  return a;
+}
+__device__ __forceinline__ void scale16(float* f, float s) {
+#pragma unroll
+  for (int i = 0; i < 16; i += 2) (F2(f[i], f[i + 1]) * F2(s)).get(f[i], f[i + 1]);
+}
+
 __device__ __forceinline__ uint32_t abs_bits(float f) { return __float_as_uint(f) & 0x7fffffffu; }
-// 16 values times inv as e4m3: finite ones or NaN.
-__device__ __forceinline__ uint4 e4m3_16(const float* f, float inv) {
+// 16 values as e4m3: finite ones or NaN.
+__device__ __forceinline__ uint4 e4m3_16(const float* f) {
   uint32_t w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    w[i] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(f[4 * i] * inv, f[4 * i + 1] * inv), __NV_SATFINITE, __NV_E4M3) |
-           ((uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(f[4 * i + 2] * inv, f[4 * i + 3] * inv), __NV_SATFINITE, __NV_E4M3) << 16);
+    w[i] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(f[4 * i], f[4 * i + 1]), __NV_SATFINITE, __NV_E4M3) |
+           ((uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(f[4 * i + 2], f[4 * i + 3]), __NV_SATFINITE, __NV_E4M3) << 16);
   return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// The same of their products with inv.
+__device__ __forceinline__ uint4 e4m3_16(float* f, float inv) {
+  scale16(f, inv);
+  return e4m3_16(f);
 }
 // What is not finite as NaN.  Rare: the empty statement keeps the compiler from doing it for every block and selecting after.
 __device__ __forceinline__ void only_finite16(float* f, bool special) {
@@ -274,8 +299,7 @@ __device__ __forceinline__ float clamp_nan(float v, float m) {
 template <class T>
 __device__ __forceinline__ void restore16(const u128& w, float scale, float* f) {
   e4m3_16_to_float(make_uint4((uint32_t)w.x, (uint32_t)(w.x >> 32), (uint32_t)w.y, (uint32_t)(w.y >> 32)), f);
-#pragma unroll
-  for (int i = 0; i < 16; ++i) f[i] *= scale;
+  scale16(f, scale);
   if (!(fabsf(scale) <= MaxOf<T>::scale)) {
     asm volatile("");
 #pragma unroll

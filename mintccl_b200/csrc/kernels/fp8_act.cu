@@ -21,39 +21,59 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// (1 + exp(-x)) / 4, whose reciprocal does not underflow before the sum overflows (an exponential below 2^-126 may be zero
-// beside the 1)
-__device__ __forceinline__ float quarter_y(float x) {
-  float e;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x * -1.4426950408889634f));
-  return __fmaf_rn(e, 0.25f, 0.25f);
+__device__ __forceinline__ float ex2_fast(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
 }
 __device__ __forceinline__ float rcp_fast(float v) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
-// 1 / (1 + exp(-x))
+// 4 / (1 + exp(-x)) of two values: the reciprocal of (1 + exp(-x)) / 4 does not underflow before the sum overflows (an
+// exponential below 2^-126 may be zero beside the 1)
+__device__ __forceinline__ F2 sigmoid4_fast(F2 x) {
+  float a, b;
+  (x * F2(-1.4426950408889634f)).get(a, b);
+  fma2(F2(ex2_fast(a), ex2_fast(b)), F2(0.25f), F2(0.25f)).get(a, b);
+  return F2(rcp_fast(a), rcp_fast(b));
+}
+// y = silu(x), 16 values
 template <bool EXACT>
-__device__ __forceinline__ float sigmoid_of(float x) {
-  if constexpr (EXACT) {
-    const float y = 1.f + expf(-x);
-    return y <= 3.4028234e38f ? 0.25f * four_over(0.25f * y) : (y != y ? y : 0.f);
-  } else {
-    return 0.25f * rcp_fast(quarter_y(x));
+__device__ __forceinline__ void silu16(const float* x, float* y) {
+#pragma unroll
+  for (int i = 0; i < 16; i += 2) {
+    if constexpr (EXACT) {
+      y[i] = silu1(x[i]);
+      y[i + 1] = silu1(x[i + 1]);
+    } else {
+      const F2 v(x[i], x[i + 1]);
+      (F2(0.25f) * v * sigmoid4_fast(v)).get(y[i], y[i + 1]);
+    }
   }
 }
+// s = 1 / (1 + exp(-x)) of two values
 template <bool EXACT>
-__device__ __forceinline__ float silu_of(float x) {
-  if constexpr (EXACT) return silu1(x);
-  else return (0.25f * x) * rcp_fast(quarter_y(x));
+__device__ __forceinline__ F2 sigmoid2(float x0, float x1) {
+  if constexpr (EXACT) {
+    auto one = [](float x) {
+      const float y = 1.f + expf(-x);
+      return y <= 3.4028234e38f ? 0.25f * four_over(0.25f * y) : (y != y ? y : 0.f);
+    };
+    return F2(one(x0), one(x1));
+  } else {
+    return F2(0.25f) * sigmoid4_fast(F2(x0, x1));
+  }
 }
 
-// 8192 x 4096 bf16, us: forward 29.7 (5.7 TB/s), gated 48 (5.6), backward 29.6 (5.7), gated 53 (5.1); a copy runs at 6.0.  What is
-// in the way is some 18 instructions an element.  U: blocks a thread has in flight; with one the ungated forms took 36 and 34,
-// with two the gated ones 53 and 62.
+// 8192 x 4096 bf16, us: forward 28.8 (5.8 TB/s), gated 45.6 (5.9), backward 28.7 (5.8), gated 49.5 (5.4); a copy runs at 6.0.
+// Multiplications go two to an instruction (29.7, 48, 29.6 and 53 one by one): the rest is some 12 an element.  U: blocks a
+// thread has in flight; with one the ungated forms took 36 and 34, with two the gated ones 53 and 62.
+// Four CTAs an SM for 16-bit types; fp32 ones have twice the words in flight and spill under that limit (8192 x 1792, gated
+// forward 38, without it 33.5).
 template <class T, int VEC, bool GATED, int U>
-__global__ void __launch_bounds__(kThreads, 4) fp8_act_fwd_kernel(Fp8ActArgs a, RowGrid grid) {
+__global__ void __launch_bounds__(kThreads, sizeof(typename T::elem) == 2 ? 4 : 0) fp8_act_fwd_kernel(Fp8ActArgs a, RowGrid grid) {
   using E = typename T::elem;
   using W = WarpSpans<T, VEC>;
   constexpr int kE = (int)sizeof(E);
@@ -78,15 +98,14 @@ __global__ void __launch_bounds__(kThreads, 4) fp8_act_fwd_kernel(Fp8ActArgs a, 
     float f[16], y[16];
     uint32_t e;
     h[u].get(f);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) y[i] = silu_of<kExact>(f[i]);
+    silu16<kExact>(f, y);
     uint4 q = encode_row16(h[u], f, &e);
     if (n > 0) *(uint4*)(a.kh.data + at + 128 * u) = q;
     if (first && p.live(u)) a.kh.scale[p.row * a.kh.s_row + (p.kb + u) * a.kh.s_col] = fp8_scale(e);
     if (GATED) {
       g[u].get(f);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) y[i] *= f[i];
+      for (int i = 0; i < 16; i += 2) (F2(y[i], y[i + 1]) * F2(f[i], f[i + 1])).get(y[i], y[i + 1]);
       q = encode_row16(g[u], f, &e);
       if (n > 0) *(uint4*)(a.ku.data + at + 128 * u) = q;
       if (first && p.live(u)) a.ku.scale[p.row * a.ku.s_row + (p.kb + u) * a.ku.s_col] = fp8_scale(e);
@@ -96,8 +115,9 @@ __global__ void __launch_bounds__(kThreads, 4) fp8_act_fwd_kernel(Fp8ActArgs a, 
   }
 }
 
-template <class T, int VEC, bool GATED, int U>
-__global__ void __launch_bounds__(kThreads) fp8_act_bwd_kernel(Fp8ActArgs a, RowGrid grid) {
+// ACT: the activation is wanted too (its values cost 16 registers, a quarter of a thread's)
+template <class T, int VEC, bool GATED, int U, bool ACT>
+__global__ void __launch_bounds__(kThreads, sizeof(typename T::elem) == 2 && VEC ? 4 : 0) fp8_act_bwd_kernel(Fp8ActArgs a, RowGrid grid) {
   using E = typename T::elem;
   using W = WarpSpans<T, VEC>;
   constexpr int kE = (int)sizeof(E);
@@ -129,21 +149,24 @@ __global__ void __launch_bounds__(kThreads) fp8_act_bwd_kernel(Fp8ActArgs a, Row
   for (int u = 0; u < U; ++u) {
     const int n = p.n(u);
     if (VEC > 0 && n <= 0) break;
-    float h[16], g[16], f[16], act[16];
+    float h[16], g[16], f[16], act[ACT ? 16 : 1];
     restore16<F32>(hq[u], hs[u], h);
     if (GATED) restore16<F32>(gq[u], gs[u], g);
     d[u].get(f);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < 16; i += 2) {
       // slope = s (1 + x (1 - s))
-      const float x = h[i], s = sigmoid_of<kExact>(x), slope = __fmaf_rn(s, __fmaf_rn(-s, x, x), s), y = x * s;
-      if (GATED) {
-        act[i] = y * g[i];
-        h[i] = f[i] * g[i] * slope;
-        g[i] = f[i] * y;
+      const F2 x(h[i], h[i + 1]), s = sigmoid2<kExact>(h[i], h[i + 1]), d2(f[i], f[i + 1]), y = x * s;
+      // x (1 - s): as x - y it is off by half a place of x, beside the 1 added to it no more than the sigmoid itself
+      const F2 rest = kExact ? fma2(s * F2(-1.f), x, x) : fma2(y, F2(-1.f), x), slope = fma2(s, rest, s);
+      if constexpr (GATED) {
+        const F2 g2(g[i], g[i + 1]);
+        if constexpr (ACT) (y * g2).get(act[i], act[i + 1]);
+        (d2 * g2 * slope).get(h[i], h[i + 1]);
+        (d2 * y).get(g[i], g[i + 1]);
       } else {
-        act[i] = y;
-        h[i] = f[i] * slope;
+        if constexpr (ACT) y.get(act[i], act[i + 1]);
+        (d2 * slope).get(h[i], h[i + 1]);
       }
     }
     d[u].set(h);
@@ -152,7 +175,7 @@ __global__ void __launch_bounds__(kThreads) fp8_act_bwd_kernel(Fp8ActArgs a, Row
       d[u].set(g);
       W::store(d[u], (uint8_t*)a.du + (p.row * a.lddu + p.c0 + 128 * u) * kE, n, stage);
     }
-    if (a.y) {
+    if constexpr (ACT) {
       d[u].set(act);
       W::store(d[u], (uint8_t*)a.y + (p.row * a.ldy + p.c0 + 128 * u) * kE, n, stage);
     }
@@ -167,7 +190,8 @@ cudaError_t act_go(const Fp8ActArgs& a, bool forward, cudaStream_t s) {
   dim3 grid;
   if (cudaError_t e = row_grid<U>(a.rows, a.cols, &g, &grid); e != cudaSuccess) return e;
   if (forward) fp8_act_fwd_kernel<T, VEC, GATED, U><<<grid, kThreads, 0, s>>>(a, g);
-  else fp8_act_bwd_kernel<T, VEC, GATED, U><<<grid, kThreads, 0, s>>>(a, g);
+  else if (a.y) fp8_act_bwd_kernel<T, VEC, GATED, U, true><<<grid, kThreads, 0, s>>>(a, g);
+  else fp8_act_bwd_kernel<T, VEC, GATED, U, false><<<grid, kThreads, 0, s>>>(a, g);
   return cudaGetLastError();
 }
 template <class T, int VEC>
