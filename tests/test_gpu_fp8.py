@@ -146,6 +146,26 @@ def test_product_with_scales_that_are_powers_of_two(size, form):
     assert N.lib().mt_gemm_fp8_error() == 0
 
 
+@pytest.mark.parametrize("form", ["fwd", "dgrad", "wgrad"])
+@pytest.mark.parametrize("size, nctas", [((600, 700, 8200), 16), ((600, 600, 8200), 16), ((1792, 4096, 6200), 0), ((1030, 4996, 9000), 0)])
+def test_product_with_a_last_wave_of_few_tiles(size, nctas, form):
+    """Long sums and one or a few tiles more than whole waves, the last of them partly behind the matrix."""
+    a, b, a64, b64 = operands(form, *size, spread=4.0)
+    c, d = (x[0].clone() for x in (a, b))
+    sc, sd = (torch.exp2(torch.round(torch.log2(x[1]))) for x in (a, b))
+    c64 = c.view(torch.float8_e4m3fn).double() * fp8._spread(sc, *c.shape, "col" if form == "wgrad" else "row").double()
+    d64 = d.view(torch.float8_e4m3fn).double() * fp8._spread(sd, *d.shape, "tile").double()
+    c64, d64 = c64.t() if form == "wgrad" else c64, d64.t() if form == "fwd" else d64
+    for dtype in (torch.float32, torch.bfloat16):
+        whole = torch.full((size[0] + 130, size[1] + 8), 7.0, device="cuda", dtype=dtype)
+        got = product(form, a, b, out=whole[:size[0], :size[1]], nctas=nctas)
+        check_product(got, a64, b64)
+        assert bool((whole[size[0]:] == 7).all()) and bool((whole[:, size[1]:] == 7).all())
+        assert torch.equal(product(form, a, b, dtype=dtype, nctas=nctas), got)
+        check_product_pow2(product(form, (c, sc), (d, sd), dtype=dtype, nctas=nctas, power_of_two=True), c64, d64)
+    assert N.lib().mt_gemm_fp8_error() == 0
+
+
 def test_scales_at_the_ends_of_the_range_and_others_than_promised():
     M, Nn, K = 2304, 2048, 384
     a, b, *_ = operands("fwd", M, Nn, K)
