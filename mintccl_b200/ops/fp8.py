@@ -352,7 +352,8 @@ def linear_fp8(x: torch.Tensor, w: torch.Tensor, w_fp8: Optional[Quantized] = No
         y = row(x) @ tile(w).T      dx = row(dy) @ tile(w)      dw = col(dy).T @ tile(x)
 
     where row, col and tile are trips through ``quantize_fp8``.  Between the passes ``x`` and ``w`` are kept in 8 bits.
-    ``w_fp8``: ``quantize_fp8(w, "tile")`` where the caller has it (one weight, several micro-batches)."""
+    ``w_fp8``: ``quantize_fp8(w, "tile")`` where the caller has it (one weight, several micro-batches); scales from elsewhere
+    must be powers of two as well (``gemm_fp8`` says what becomes of others)."""
     if x.dim() < 1 or w.dim() != 2 or x.shape[-1] != w.shape[1]:
         raise ValueError("x must be [..., K] and w [N, K]")
     _check_float(x, "x")
