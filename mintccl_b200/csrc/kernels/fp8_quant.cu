@@ -61,7 +61,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(typename T::elem) == 2 && !RO
   // rows of this thread that exist, of four; where the first is in a payload, and the distance to the next
   const int64_t r0 = (int64_t)rt * 128 + g, q0 = r0 * a.ldq + c0, qstep = 32 * a.ldq;
   const int live = (int)min((int64_t)4, max((int64_t)0, (a.rows - r0 + 31) >> 5));
-  const bool put = c0 < a.ldq;
+  const bool put = n > 0;   // a row's padding to 16 bytes is zeros; what lies behind it, up to the next row, is not this matrix's
   Span16<T, VEC> in[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i)

@@ -641,3 +641,27 @@ def test_layers_on_two_streams_at_once():
     for i in range(2):
         for r in got[i]:
             assert all(torch.equal(a, b) for a, b in zip(r, sets[i][3]))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape, pitch", [((5, 100), 512), ((130, 16), 256), ((129, 1), 128), ((3, 250), 320), ((40, 129), 144), ((129, 384), 1024)])
+def test_encoding_leaves_what_lies_between_payload_rows(shape, pitch, dtype):
+    """The C entry with payload rows further apart than their padding to 16 bytes, as in a slice of a wider buffer: nothing
+    else is written, behind the last row either."""
+    rows, cols = shape
+    pad = fp8._up16(cols)
+    base = values((rows, cols + 1), dtype, seed=cols).cuda()
+    for x in (base[:, :cols], base[:, 1:], base[:, :cols].contiguous()):
+        for blocks in (("row",), ("col",), ("tile",), ("row", "col"), ("row", "tile"), ("col", "tile"), ("row", "col", "tile")):
+            bufs, ptrs = {}, [0] * 6
+            for b in blocks:
+                bufs[b] = torch.full((rows + 1, pitch), 0xab, device="cuda", dtype=torch.uint8), fp8._new_scale(rows, cols, b, "cuda")
+                at = 2 * ("row", "col", "tile").index(b)
+                ptrs[at:at + 2] = (t.data_ptr() for t in bufs[b])
+            rc = N.lib().mt_fp8_quantize(N.raw_stream(0), fp8.DTYPES[dtype], x.data_ptr(), x.stride(0), rows, cols, pitch,
+                                         *(p or None for p in ptrs))
+            assert rc == 0, N.last_error()
+            for b, (data, scale) in bufs.items():
+                same_encoding((data[:rows, :cols], scale), x, b)
+                assert bool((data[:rows, cols:pad] == 0).all())
+                assert bool((data[:rows, pad:] == 0xab).all()) and bool((data[rows] == 0xab).all()), (b, blocks)
