@@ -102,9 +102,7 @@ def _backward(h: Saved8, u: Optional[Saved8], dy: torch.Tensor, act: bool):
     if dh.numel():
         pitch, ins, live = _up16(cols), [], []
         for k in kept:
-            data, p = _payload(k.data, "the saved payload", vectors=True)
-            if p != pitch:      # a copy of what was kept may come back with rows further apart
-                data = _new_payload(rows, cols, data).copy_(data)
+            data, _ = _payload(k.data, "the saved payload", vectors=True, apart=pitch)     # what was kept may come back otherwise
             live.append(data)
             ins += [data.data_ptr(), k.scale.data_ptr(), *k.scale.stride()]
         if u is None:

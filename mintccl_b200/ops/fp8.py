@@ -101,21 +101,22 @@ def _rows(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
     return t, ld if rows > 1 else 0
 
 
-def _payload(t: torch.Tensor, name: str, vectors: bool = False) -> Tuple[torch.Tensor, int]:
+def _payload(t: torch.Tensor, name: str, vectors: bool = False, apart: int = 0) -> Tuple[torch.Tensor, int]:
     """A payload as the kernels take it, and the bytes between its rows: copied where its rows are not on 16-byte boundaries,
-    or (``vectors``: the kernel reads whole ones) where the last row's padding is not there to be read."""
+    not ``apart`` bytes apart (the kernel wants its payloads alike), or (``vectors``: the kernel reads whole ones) where the
+    last row's padding is not there to be read."""
     if t.dtype not in _U8 or t.dim() != 2:
         raise ValueError(f"{name} must be a 2-D uint8 or float8_e4m3fn tensor")
     (rows, cols), (pitch, inner) = t.shape, t.stride()
     if rows <= 1:
         pitch = _up16(cols)
-    if (cols <= 1 or inner == 1) and pitch % 16 == 0 and pitch >= cols and t.data_ptr() % 16 == 0:
+    if (cols <= 1 or inner == 1) and pitch % 16 == 0 and pitch >= cols and t.data_ptr() % 16 == 0 and apart in (0, pitch):
         if not vectors or cols % 16 == 0:
             return t, pitch
         if t.storage_offset() + (rows - 1) * pitch + _up16(cols) <= t.untyped_storage().nbytes():
             return t, pitch
     buf = _new_payload(rows, cols, t)
-    buf.copy_(t.view(torch.uint8))
+    buf.copy_(t.view(torch.uint8))      # bytes: from float8 a copy would convert
     return buf, _up16(cols)
 
 

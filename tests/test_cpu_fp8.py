@@ -284,3 +284,20 @@ def test_mlp_refuses_unknown_checkpoints():
         world_size = 1
     with pytest.raises(ValueError):
         tp_mlp.TensorParallelMLP(Comm(), 128, 256, 256, checkpoint="fp4")
+
+
+@pytest.mark.parametrize("kind", [torch.uint8, torch.float8_e4m3fn], ids=str)
+def test_payloads_are_copied_by_their_bytes(kind):
+    """Where a kernel cannot take a payload as it lies, it gets a copy of the bytes, whatever type they have."""
+    g = torch.Generator().manual_seed(4)
+    wide = torch.randint(0, 256, (7, 96), generator=g, dtype=torch.uint8)
+    for t, apart in ((wide[:, :30], 32), (wide[:, 3:33], 0), (wide[:, :60:2], 0), (wide[:1, 1:31], 0), (wide[:, 64:94], 32),
+                     (wide.t()[:30], 0)):
+        got, pitch = fp8._payload(t.view(kind) if t.is_contiguous() else wide.view(kind).as_strided(t.shape, t.stride(), t.storage_offset()),
+                                  "payload", vectors=True, apart=apart)
+        assert pitch == 32 if t.shape[1] == 30 else pitch % 16 == 0
+        assert torch.equal(got.view(torch.uint8), t)
+    kept = wide[:, :32].view(kind)
+    assert fp8._payload(kept, "payload", vectors=True)[0] is kept
+    again, pitch = fp8._payload(kept, "payload", vectors=True, apart=32)
+    assert pitch == 32 and torch.equal(again.view(torch.uint8), wide[:, :32])

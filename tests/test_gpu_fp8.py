@@ -665,3 +665,26 @@ def test_encoding_leaves_what_lies_between_payload_rows(shape, pitch, dtype):
                 same_encoding((data[:rows, :cols], scale), x, b)
                 assert bool((data[:rows, cols:pad] == 0).all())
                 assert bool((data[:rows, pad:] == 0xab).all()) and bool((data[rows] == 0xab).all()), (b, blocks)
+
+
+@pytest.mark.parametrize("kind", [torch.uint8, torch.float8_e4m3fn], ids=str)
+@pytest.mark.parametrize("cols", [30, 128, 1000])
+def test_activation_gradient_from_payloads_in_another_layout(cols, kind):
+    """Kept payloads that come back as float8, and as a slice of a wider tensor: the same gradients."""
+    gate, up, dy = torch.randn(3, 40, cols, device="cuda")
+    _, saved = c8.swiglu8_forward(gate, up)
+    want = c8.swiglu8_backward(saved, dy, act=True)
+    alone = c8.silu8_backward(saved[0], dy, act=True)
+
+    def moved(k, left):
+        wide = torch.full((40, 2048), 0x55, device="cuda", dtype=torch.uint8)
+        wide[:, left:left + cols] = k.data
+        return k._replace(data=wide.view(kind)[:, left:left + cols])
+
+    for left in (0, 16, 7):
+        other = tuple(moved(k, left) for k in saved)
+        for a, b in zip(c8.swiglu8_backward(other, dy, act=True), want):
+            assert torch.equal(a, b)
+        for a, b in zip(c8.silu8_backward(other[0], dy, act=True), alone):
+            assert torch.equal(a, b)
+        assert torch.equal(other[0].restore(), saved[0].restore())
