@@ -25,8 +25,8 @@
 //   warp 9       (leader) issues tcgen05.mma: four a stage; commits to "stage empty" and "accumulator full" of both CTAs
 //   warps 10, 11 scales: the products sa * sb of a block for the CTA's rows and both halves, blocks ahead of their use
 //
-// Measured (bf16 out, scales of any value / powers of two): 8192 x 1792 x 4096 66 / 51 us, 8192 x 4096 x 4096 138 / 100 (2.0 / 2.75
-// PFLOP/s).  With scales of any value the sum warps' chain is the bound: about 400 cycles a block and 128 columns, where the
+// Measured (bf16 out, scales of any value / powers of two): 8192 x 1792 x 4096 63 / 50 us, 8192 x 4096 x 4096 131 / 100 (2.1 / 2.75
+// PFLOP/s).  With scales of any value the sum warps' chain is the bound: about 380 cycles a block and 128 columns, where the
 // tensor core and its operands' way through shared memory need 340.  A product's loads are 7.2 % of the HBM's time then.
 // Tiles of 128 columns with four accumulators: with 256 columns and two, the tensor core waits for the sums after every
 // block (890 cycles for the 256); POW2 has tiles of 256, whose only accumulator is drained once a tile.
@@ -247,7 +247,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_fp8_kernel(const __grid_cons
         mbar_init(&ctl->empty[s], 1);
       }
       for (int s = 0; s < ACC; ++s) {
-        mbar_init(&ctl->acc_full[s], 1);
+        mbar_init(&ctl->acc_full[s], POW2 ? 1 : 2);   // the products; of a block also the CTA's own scale warp
         mbar_init(&ctl->acc_empty[s], PAIR ? 2 * kSumWarps : kSumWarps);   // the leader's counts both CTAs
       }
       mbar_init(&ctl->drain, 1);
@@ -320,13 +320,15 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_fp8_kernel(const __grid_cons
           // an accumulator is one block's, with POW2 a whole tile's
           const bool fresh = !POW2 || kb == 0, done = !POW2 || kb + 1 == kblocks;
           // both probes in flight at once: each takes some 230 cycles beside the tensor core's own shared-memory traffic
-          const bool drained = !fresh || mbar_test(&ctl->acc_empty[b], bph ^ 1), loaded = mbar_test(&ctl->full[s], ph);
+          const bool drained = !fresh || mbar_test(&ctl->acc_empty[b], bph ^ 1),
+                     loaded = PAIR ? mbar_test_cluster(&ctl->full[s], ph) : mbar_test(&ctl->full[s], ph);
           if (!__all_sync(0xffffffffu, drained && loaded) &&
               ((fresh && !wait_bar_warp(&ctl->acc_empty[b], bph ^ 1, abort_flag, a.timeout_ns)) ||
-               !wait_bar_warp(&ctl->full[s], ph, abort_flag, a.timeout_ns))) {
+               !wait_bar_warp<PAIR>(&ctl->full[s], ph, abort_flag, a.timeout_ns))) {
             ok = false;
             break;
           }
+          if (PAIR) fence_acquire_cluster_smem();
           tc_fence_after();
           const uint64_t da = TA ? make_smem_desc_mn_sw128(sA + s * A_BYTES, 128 * BK) : make_smem_desc_sw128(sA + s * A_BYTES);
           const uint64_t db = !TB          ? make_smem_desc_sw128(sB + s * B_BYTES)
@@ -373,9 +375,13 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_fp8_kernel(const __grid_cons
       wait_bar_warp(&ctl->drain, 0, abort_flag, a.timeout_ns);
     } else if (warp >= kSumWarps + 2) {
       // ---------------------------------------------------------- scales: one warp for even blocks, one for odd; a lane has
-      // four rows, 32 apart.  They count on the stage's "full" barrier: whoever sees the block's accumulator sees them too.
-      // A slot is free when its stage is: the sums are at most ACC + STAGES blocks behind.
-      static_assert(POW2 || ACC + STAGES < kScaleSlots, "slots of the scales");
+      // four rows, 32 apart.  They count on the stage's "full" barrier, so that no block overtakes its scales: a slot is free
+      // when its stage is, the sums are at most ACC + STAGES blocks behind and have used what was there.  With POW2 the tensor
+      // core reads the bytes of both CTAs: the leader, which waits for "full" and issues for both, sees them by the fences of
+      // the two.  Factors are for the sum warps of the same CTA: they count on its "accumulator full" barrier as well, once the
+      // block before on that accumulator has come out.  (A barrier of their own for the sums to wait on, on whose time
+      // everything hangs: 8192 x 4096 x 4096 136 us, with one for four blocks 142, this way 131.)
+      static_assert(POW2 || (ACC + STAGES < kScaleSlots && ACC == 4), "slots of the scales, their accumulators");
       const int w = warp - kSumWarps - 2;
       const uint32_t full_leader = map_to_cta(smem_u32(&ctl->full[0]), 0);
       uint32_t s = w, ph = 0, pos = 0;   // stage of this warp's next block, and the tile's first block among all
@@ -421,8 +427,14 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_fp8_kernel(const __grid_cons
             }
             __syncwarp();
             if (lane == 0) {
-              if (PAIR) mbar_arrive_cluster(full_leader + s * 8);
+              if (PAIR) mbar_arrive_cluster_release(full_leader + s * 8);
               else mbar_arrive(&ctl->full[s]);
+            }
+            if constexpr (!POW2) {
+              const uint32_t n = pos + kb + 2 * j, b = n & (ACC - 1);
+              ok = ok && wait_bar_warp(&ctl->acc_full[b], (n / ACC & 1) ^ 1, abort_flag, a.timeout_ns);
+              if (ok && lane == 0) mbar_arrive(&ctl->acc_full[b]);
+              __syncwarp();
             }
             s += 2;
             if (s >= STAGES) {

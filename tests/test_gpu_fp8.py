@@ -688,3 +688,30 @@ def test_activation_gradient_from_payloads_in_another_layout(cols, kind):
         for a, b in zip(c8.silu8_backward(other[0], dy, act=True), alone):
             assert torch.equal(a, b)
         assert torch.equal(other[0].restore(), saved[0].restore())
+
+
+@pytest.mark.parametrize("form", ["fwd", "dgrad", "wgrad"])
+@pytest.mark.parametrize("size", [(2304, 2048, 4100), (700, 300, 5000), (64, 256, 8192)], ids=["pairs", "single", "shared"])
+def test_every_block_takes_its_own_scales(size, form):
+    """Neighbouring blocks' scales are powers of two far apart and every call has others in their places: a block that met
+    another block's, another row's or the last call's would be off by a factor.  The calls follow one another unwatched."""
+    a, b, *_ = operands(form, *size)
+    M, Nn, K = size
+    sets = []
+    for i in range(6):
+        at = lambda n, step: torch.arange(n, device="cuda").mul(step).add(5 * i).remainder(23).sub(11)               # noqa: E731
+        # [M, blocks of K] and [blocks of N, blocks of K]
+        sa = torch.exp2((at(M, 7)[:, None] + at(-(-K // 128), 9)[None]).float())
+        sb = torch.exp2((at(-(-Nn // 128), 5)[:, None] - at(-(-K // 128), 4)[None]).float())
+        sets.append((a[1].new_empty(a[1].shape).copy_(sa.t() if form == "wgrad" else sa), sb if form == "fwd" else sb.t()))
+    torch.cuda.synchronize()
+    outs = [[product(form, (a[0], sa), (b[0], sb), dtype=torch.float32, power_of_two=pow2) for sa, sb in sets for _ in range(4)]
+            for pow2 in (False, True)]
+    for i, (sa, sb) in enumerate(sets):
+        a64 = a[0].view(torch.float8_e4m3fn).double() * fp8._spread(sa, *a[0].shape, "col" if form == "wgrad" else "row").double()
+        b64 = b[0].view(torch.float8_e4m3fn).double() * fp8._spread(sb, *b[0].shape, "tile").double()
+        a64, b64 = a64.t() if form == "wgrad" else a64, b64.t() if form == "fwd" else b64
+        for got, check in zip(outs, (check_product, check_product_pow2)):
+            check(got[4 * i], a64, b64)
+            assert all(torch.equal(got[4 * i + j], got[4 * i]) for j in range(1, 4))
+    assert N.lib().mt_gemm_fp8_error() == 0
