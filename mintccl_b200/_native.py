@@ -147,6 +147,7 @@ def lib():
     sig("mt_gemm_fp8", i32, vp, vp, i64, vp, i64, i64, vp, i64, vp, i64, i64, vp, i64, i32, i64, i64, i64, i32, i32, i32)
     sig("mt_fp8_packed", i32, vp, i32, cp)
     sig("mt_gemm_fp8_error", i32)
+    sig("mt_test_gemm_fp8_expire", i32, vp)
     sig("mt_test_wait_timeout", i32, vp, vp)
     sig("mt_test_one_rank_args", i32, u64, vp, u64, C.POINTER(u64))
     sig("mt_find_ring", i32, C.POINTER(C.c_double), i32, ip)

@@ -265,6 +265,15 @@ int mt_fp8_packed(void* stream, int op, const int64_t* v) {
   }
 }
 
-int mt_gemm_fp8_error(void) { return mt::fp8_gemm_error(); }
+int mt_gemm_fp8_error(void) {
+  return guarded([&]() -> int {
+    int expired = 0;
+    return launched(mt::fp8_gemm_error(&expired), "fp8 gemm status") ? -1 : expired;
+  });
+}
+
+int mt_test_gemm_fp8_expire(void* stream) {
+  return guarded([&]() -> int { return launched(mt::launch_fp8_gemm_expire((cudaStream_t)stream), "launch"); });
+}
 
 }  // extern "C"

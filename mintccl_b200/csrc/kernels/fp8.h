@@ -62,6 +62,8 @@ struct Fp8GemmArgs {
 // CTAs that share a tile's blocks along K, at most as many as there are blocks; nctas = split * tiles if it is not 1.
 // pow2: all scales are powers of two (looked at with pair only).
 cudaError_t launch_fp8_gemm(int bn, bool pair, bool pow2, int split, bool ta, bool tb, const Fp8GemmArgs& a, int nctas, cudaStream_t s);
-int fp8_gemm_error();   // 1 after a wait of the kernel expired (synchronises), -1 on a CUDA error
+// *expired = 1 if a wait of the product expired on the current device since the last call (waits for the device).
+cudaError_t fp8_gemm_error(int* expired);
+cudaError_t launch_fp8_gemm_expire(cudaStream_t s);   // a kernel whose wait expires
 
 }  // namespace mt

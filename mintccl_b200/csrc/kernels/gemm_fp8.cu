@@ -31,8 +31,8 @@
 // Tiles of 128 columns with four accumulators: with 256 columns and two, the tensor core waits for the sums after every
 // block (890 cycles for the 256); POW2 has tiles of 256, whose only accumulator is drained once a tile.
 //
-// Every wait is bounded; on expiry the CTA raises its abort flag, all roles leave their loops, TMEM is freed and a
-// device-side error word is set for the host.
+// Every wait is bounded; on expiry the CTA raises its abort flag, all roles leave their loops, TMEM is freed and the
+// device's error word is set, until fp8_gemm_error reads it.
 //
 // The reference has no compute kernels (README.md:5 only asks that collectives fuse with others).
 #include <cuda.h>
@@ -575,6 +575,15 @@ cudaError_t go_form(bool ta, bool tb, const Fp8GemmArgs& a, int cluster, int nct
   return tb ? go<BN, PAIR, POW2, false, true>(a, cluster, nctas, s) : go<BN, PAIR, POW2, false, false>(a, cluster, nctas, s);
 }
 
+// Self test: a wait that nothing ends, for 1 ms.
+__global__ void expire_kernel() {
+  __shared__ uint64_t bar;
+  __shared__ int abort;
+  mbar_init(&bar, 1);
+  abort = 0;
+  if (!wait_bar(&bar, 0, &abort, 1000000ull)) atomicExch(&g_error, 1);
+}
+
 }  // namespace fp8g
 
 cudaError_t launch_fp8_gemm(int bn, bool pair, bool pow2, int split, bool ta, bool tb, const Fp8GemmArgs& a, int nctas, cudaStream_t s) {
@@ -585,10 +594,17 @@ cudaError_t launch_fp8_gemm(int bn, bool pair, bool pow2, int split, bool ta, bo
   return fp8g::go_form<128, false, false>(ta, tb, a, split, nctas, s);
 }
 
-int fp8_gemm_error() {
-  int v = 0;
-  if (cudaMemcpyFromSymbol(&v, fp8g::g_error, sizeof(int)) != cudaSuccess) return -1;
-  return v;
+cudaError_t fp8_gemm_error(int* expired) {
+  cudaError_t e = cudaDeviceSynchronize();   // products on every stream, those too that the copy would not wait for
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbol(expired, fp8g::g_error, sizeof(int));
+  const int none = 0;
+  if (e == cudaSuccess && *expired) e = cudaMemcpyToSymbol(fp8g::g_error, &none, sizeof(int));
+  return e;
+}
+
+cudaError_t launch_fp8_gemm_expire(cudaStream_t s) {
+  fp8g::expire_kernel<<<1, 1, 0, s>>>();
+  return cudaGetLastError();
 }
 
 }  // namespace mt

@@ -191,11 +191,13 @@ int mt_gemm_fp8(void* stream, const void* A, int64_t lda, const void* sa, int64_
 enum { MT_FP8_QUANTIZE = 0, MT_FP8_DEQUANTIZE, MT_FP8_ACT_FORWARD, MT_FP8_ACT_BACKWARD, MT_FP8_GEMM, MT_FP8_LINEAR_FORWARD,
        MT_FP8_LINEAR_BACKWARD };
 int mt_fp8_packed(void* stream, int op, const int64_t* args);
-// 1 after a bounded wait of mt_gemm_fp8 expired (synchronises; the result of that call is then invalid), 0 otherwise
+// 1 if a bounded wait of a product (mt_gemm_fp8, the linear layer's) expired on the current device since this was last asked:
+// the result of such a call is invalid.  0 otherwise, -1 on an error.  Waits for the device.
 int mt_gemm_fp8_error(void);
 
 // ---- device-wait self test: a wait nothing satisfies must time out and report, not hang -----------
 int mt_test_wait_timeout(MtComm* c, void* stream);
+int mt_test_gemm_fp8_expire(void* stream);   // the same for the products with block scales, after 1 ms
 // what the product of a one-rank plan is launched with (no GPU): out = {time limit in ns, status record, rank}
 int mt_test_one_rank_args(uint64_t timeout_ns, void* heap, uint64_t status_off, uint64_t* out);
 

@@ -11,13 +11,16 @@ which the block's largest finite magnitude is at most 448, the largest e4m3 valu
 it is exact, so the rounding to e4m3 is the only one.  Infinities and NaN become NaN and leave the rest of their block as it
 is.  ``gemm_fp8`` takes scales of any value, as checkpoints bring them.
 
+Waits inside the product kernels are bounded, as in the collectives: one that runs out ends the kernel, whose output is then
+not valid.  ``check`` says so, as ``Communicator.check`` does for collectives.
+
 MXFP8 (``ops/mxfp8.py``) has a scale of 8 bits for each 32 elements instead, which the tensor cores apply themselves.
 The reference has no fp8 path; it is on its roadmap (README.md:58-60).
 """
 from __future__ import annotations
 
 import struct
-from typing import List, Optional, Sequence, Tuple
+from typing import List, Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -261,6 +264,20 @@ def gemm_fp8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: t
           b_scale.data_ptr(), *((sb_c, sb_r) if tb else (sb_r, sb_c)), out.data_ptr(), ldc, DTYPES[out.dtype], M, Nn, K, int(ta), int(tb),
           nctas, int(power_of_two))
     return out
+
+
+def check(device: Optional[Union[int, str, torch.device]] = None) -> None:
+    """Raises ``RuntimeError`` if a wait inside a product (``gemm_fp8``, either pass of ``linear_fp8``) ran out on ``device`` (the
+    current one by default) since the last check: something that was returned since then is not valid.  Waits for all work on
+    the device: for the end of a step, not for a captured one."""
+    if device is not None:
+        with torch.cuda.device(device):
+            return check()
+    rc = N.lib().mt_gemm_fp8_error()
+    if rc < 0:
+        raise RuntimeError(f"mt_gemm_fp8_error: {N.last_error()}")
+    if rc:
+        raise RuntimeError("a wait inside a block-scaled product ran out: results since the last check are not valid")
 
 
 # ---- the linear layer ----------------------------------------------------------------------------------------------

@@ -301,3 +301,14 @@ def test_payloads_are_copied_by_their_bytes(kind):
     assert fp8._payload(kept, "payload", vectors=True)[0] is kept
     again, pitch = fp8._payload(kept, "payload", vectors=True, apart=32)
     assert pitch == 32 and torch.equal(again.view(torch.uint8), wide[:, :32])
+
+
+def test_a_wait_that_ran_out_is_reported(monkeypatch):
+    import types
+    for rc, raises in ((0, False), (1, True), (-1, True)):
+        monkeypatch.setattr(fp8.N, "lib", lambda: types.SimpleNamespace(mt_gemm_fp8_error=lambda: rc, mt_last_error=lambda: b"why"))
+        if raises:
+            with pytest.raises(RuntimeError, match="ran out" if rc > 0 else "why"):
+                fp8.check()
+        else:
+            fp8.check()

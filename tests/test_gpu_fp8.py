@@ -715,3 +715,16 @@ def test_every_block_takes_its_own_scales(size, form):
             check(got[4 * i], a64, b64)
             assert all(torch.equal(got[4 * i + j], got[4 * i]) for j in range(1, 4))
     assert N.lib().mt_gemm_fp8_error() == 0
+
+
+def test_a_wait_that_runs_out_is_reported_once():
+    """A wait that nothing ends (1 ms), on a stream that the default one does not wait for."""
+    fp8.check()
+    s = torch.cuda.Stream()
+    assert N.lib().mt_test_gemm_fp8_expire(s.cuda_stream) == 0
+    with pytest.raises(RuntimeError, match="ran out"):
+        fp8.check("cuda:0")
+    fp8.check(0)
+    a, b, a64, b64 = operands("fwd", 300, 200, 400)
+    check_product(product("fwd", a, b), a64, b64)
+    fp8.check()
