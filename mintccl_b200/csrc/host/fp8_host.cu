@@ -247,17 +247,17 @@ int mt_fp8_packed(void* stream, int op, const int64_t* v) {
       const int64_t T = v[3], K = v[4], N = v[8], ldq = (K + 15) / 16 * 16;
       if (mt_fp8_quantize(stream, (int)v[0], p(1), v[2], T, K, ldq, p(9), p(10), nullptr, nullptr, p(11), p(12))) return -1;
       if (v[6] && mt_fp8_quantize(stream, (int)v[5], p(6), v[7], N, K, v[14], nullptr, nullptr, nullptr, nullptr, p(13), p(15))) return -1;
-      return gemm(stream, p(9), ldq, p(10), 1, T, p(13), v[14], p(15), v[16], v[17], p(18), N, (int)v[0], T, N, K, 0, 0, 0, true);
+      return gemm(stream, p(9), ldq, p(10), 1, T, p(13), v[14], p(15), v[16], v[17], p(18), N, (int)v[0], T, N, K, 0, 0, 0, v[19] != 0);
     }
     case MT_FP8_LINEAR_BACKWARD: {
       const int64_t T = v[3], N = v[4], K = v[5], ldq = (N + 15) / 16 * 16, ldx = (K + 15) / 16 * 16;
-      const bool want_x = v[13] != 0, want_w = v[18] != 0;
+      const bool want_x = v[13] != 0, want_w = v[18] != 0, pow2 = v[20] != 0;
       if (mt_fp8_quantize(stream, (int)v[0], p(1), v[2], T, N, ldq, want_x ? p(6) : nullptr, want_x ? p(7) : nullptr,
                           want_w ? p(14) : nullptr, want_w ? p(15) : nullptr, nullptr, nullptr))
         return -1;
-      if (want_x && gemm(stream, p(6), ldq, p(7), 1, T, p(8), v[9], p(10), v[12], v[11], p(13), K, (int)v[0], T, K, N, 0, 1, 0, true))
+      if (want_x && gemm(stream, p(6), ldq, p(7), 1, T, p(8), v[9], p(10), v[12], v[11], p(13), K, (int)v[0], T, K, N, 0, 1, 0, pow2))
         return -1;
-      if (want_w && gemm(stream, p(14), ldq, p(15), 1, N, p(16), ldx, p(17), 1, (K + 127) / 128, p(18), K, (int)v[19], N, K, T, 1, 1, 0, true))
+      if (want_w && gemm(stream, p(14), ldq, p(15), 1, N, p(16), ldx, p(17), 1, (K + 127) / 128, p(18), K, (int)v[19], N, K, T, 1, 1, 0, pow2))
         return -1;
       return 0;
     }

@@ -182,11 +182,11 @@ int mt_gemm_fp8(void* stream, const void* A, int64_t lda, const void* sa, int64_
 // powers of two, and what is not counts as NaN; ctypes takes 3 us to convert twenty
 // arguments one by one), and the two passes of a linear layer, each of them all of its kernels in one call.
 //   MT_FP8_LINEAR_FORWARD   dtype, x, ldx, T, K, w_dtype, w (0: encoded already), ldw, N, xr_data, xr_scale, xt_data, xt_scale
-//                           (both 0: not wanted), w_data, ldwq, w_scale, w_srow, w_scol, y
+//                           (both 0: not wanted), w_data, ldwq, w_scale, w_srow, w_scol, y, power_of_two
 //       payloads of x are ceil16(K) bytes a row, xr and xt its row blocks and tiles; w's tiles are written if w is given;
 //       y [T, N] of x's dtype, contiguous
 //   MT_FP8_LINEAR_BACKWARD  dtype, dy, lddy, T, N, K, r_data, r_scale, w_data, ldwq, w_scale, w_srow, w_scol, dx (0: none),
-//                           c_data, c_scale, xt_data, xt_scale, dw (0: none), w_dtype
+//                           c_data, c_scale, xt_data, xt_scale, dw (0: none), w_dtype, power_of_two
 //       r and c: room for the row and column blocks of dy [T, N], ceil16(N) bytes a row; dx [T, K] and dw [N, K] contiguous
 enum { MT_FP8_QUANTIZE = 0, MT_FP8_DEQUANTIZE, MT_FP8_ACT_FORWARD, MT_FP8_ACT_BACKWARD, MT_FP8_GEMM, MT_FP8_LINEAR_FORWARD,
        MT_FP8_LINEAR_BACKWARD };

@@ -294,7 +294,7 @@ def _room(nbytes: int) -> int:
 
 class _LinearFp8(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w, w_data, w_scale, keep):
+    def forward(ctx, x, w, w_data, w_scale, keep, power_of_two):
         # keep: the weight has a gradient, which contracts over the tokens; what is kept of x for it are tiles, in 8 bits
         n, k = w.shape
         x2, ldx = _rows(x if x.dim() == 2 else x.reshape(-1, k))
@@ -306,7 +306,7 @@ class _LinearFp8(torch.autograd.Function):
         size = ws + (4 * -(-n // BLOCK) * kb if own else 0)
         kept = x2.new_empty(size, dtype=torch.uint8) if size else None
         base = kept.data_ptr() if size else 0
-        ctx.sizes = t, n, k, xs, wd, ws, size, x.dtype, w.dtype
+        ctx.sizes = t, n, k, xs, wd, ws, size, x.dtype, w.dtype, power_of_two
         ctx.save_for_backward(kept, w_data, w_scale)
         y = x2.new_empty((t, n) if x.dim() == 2 else (*x.shape[:-1], n))
         if own:
@@ -319,7 +319,7 @@ class _LinearFp8(torch.autograd.Function):
             rows = x2.new_empty(_room(t * pk) + 4 * t * kb, dtype=torch.uint8)      # x's row blocks, for this product only
             at = rows.data_ptr()
             _call(LINEAR_FORWARD, y.get_device(), DTYPES[x.dtype], x2.data_ptr(), ldx, t, k, DTYPES[w.dtype], wq[0], wq[1], n, at,
-                  at + _room(t * pk), base if keep else 0, base + xs if keep else 0, *wq[2:], y.data_ptr())
+                  at + _room(t * pk), base if keep else 0, base + xs if keep else 0, *wq[2:], y.data_ptr(), int(power_of_two))
         elif own:
             _call(QUANTIZE, y.get_device(), DTYPES[w.dtype], wq[0], wq[1], n, k, pk, 0, 0, 0, 0, wq[2], wq[4])
         return y
@@ -328,7 +328,7 @@ class _LinearFp8(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         kept, w_data, w_scale = ctx.saved_tensors
-        t, n, k, xs, wd, ws, size, x_dtype, w_dtype = ctx.sizes
+        t, n, k, xs, wd, ws, size, x_dtype, w_dtype, power_of_two = ctx.sizes
         want_x, want_w = ctx.needs_input_grad[:2]
         if not _native(dy):
             raise ValueError("the gradient must be a plain CUDA tensor, and nobody recording")
@@ -358,20 +358,24 @@ class _LinearFp8(torch.autograd.Function):
             tmp = dy2.new_empty(cs + (4 * -(-t // BLOCK) * n if want_w else 0), dtype=torch.uint8)
             at = tmp.data_ptr()
             _call(LINEAR_BACKWARD, dy2.get_device(), DTYPES[x_dtype], dy2.data_ptr(), ld, t, n, k, at, at + rs, *wq,
-                  dx.data_ptr() if want_x else 0, at + cd, at + cs, base, base + xs, dw.data_ptr() if want_w else 0, DTYPES[w_dtype])
+                  dx.data_ptr() if want_x else 0, at + cd, at + cs, base, base + xs, dw.data_ptr() if want_w else 0, DTYPES[w_dtype],
+                  int(power_of_two))
         elif want_w:
             dw.zero_()
-        return dx, dw, None, None, None
+        return dx, dw, None, None, None, None
 
 
-def linear_fp8(x: torch.Tensor, w: torch.Tensor, w_fp8: Optional[Quantized] = None) -> torch.Tensor:
+def linear_fp8(x: torch.Tensor, w: torch.Tensor, w_fp8: Optional[Quantized] = None, power_of_two: bool = True) -> torch.Tensor:
     """``x [..., K] @ w[N, K].T`` through 8 bits, in ``x``'s type, with both gradients:
 
         y = row(x) @ tile(w).T      dx = row(dy) @ tile(w)      dw = col(dy).T @ tile(x)
 
     where row, col and tile are trips through ``quantize_fp8``.  Between the passes ``x`` and ``w`` are kept in 8 bits.
-    ``w_fp8``: ``quantize_fp8(w, "tile")`` where the caller has it (one weight, several micro-batches); scales from elsewhere
-    must be powers of two as well (``gemm_fp8`` says what becomes of others)."""
+    ``w_fp8``: ``quantize_fp8(w, "tile")`` where the caller has it (one weight, several micro-batches), or a checkpoint's tiles.
+
+    ``power_of_two``: that of ``gemm_fp8`` for the three products.  False where ``w_fp8`` has scales that are not (large
+    products make NaN of them otherwise), or where the rounding of sums matters more than a fifth of the time: the tensor core
+    truncates a sum to 32 bits at every 32 products, without it each block of 128 is rounded to nearest."""
     if x.dim() < 1 or w.dim() != 2 or x.shape[-1] != w.shape[1]:
         raise ValueError("x must be [..., K] and w [N, K]")
     _check_float(x, "x")
@@ -385,4 +389,4 @@ def linear_fp8(x: torch.Tensor, w: torch.Tensor, w_fp8: Optional[Quantized] = No
     data, scale = w_fp8 if w_fp8 is not None else (None, None)
     if data is not None:
         _check_encoded(data, scale, tuple(w.shape), w)
-    return _LinearFp8.apply(x, w, data, scale, torch.is_grad_enabled() and w.requires_grad)
+    return _LinearFp8.apply(x, w, data, scale, torch.is_grad_enabled() and w.requires_grad, power_of_two)

@@ -728,3 +728,21 @@ def test_a_wait_that_runs_out_is_reported_once():
     a, b, a64, b64 = operands("fwd", 300, 200, 400)
     check_product(product("fwd", a, b), a64, b64)
     fp8.check()
+
+
+def test_layer_with_a_weight_whose_scales_have_any_value():
+    """A checkpoint's tiles, at a size where the products run on pairs (and would make NaN of them): any value has to be said."""
+    T, K, Nn = 2304, 1200, 2050
+    g = torch.Generator(device="cuda").manual_seed(11)
+    x = torch.randn(T, K, generator=g, device="cuda", dtype=torch.bfloat16).requires_grad_(True)
+    dy = torch.randn(T, Nn, generator=g, device="cuda", dtype=torch.bfloat16)
+    w = torch.randn(Nn, K, generator=g, device="cuda").requires_grad_(True)
+    data, scale = fp8.quantize_fp8(w, "tile")
+    scale = scale * (torch.rand(scale.shape, generator=g, device="cuda") + 0.5)
+    w64 = data.view(torch.float8_e4m3fn).double() * fp8._spread(scale, Nn, K, "tile").double()
+    y = fp8.linear_fp8(x, w, (data, scale), power_of_two=False)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    check_product(y.detach(), trip(x, "row"), w64.t())
+    check_product(dx, trip(dy, "row"), w64)
+    check_product(dw, trip(dy, "col").t(), trip(x, "tile"))
+    fp8.check()
