@@ -26,7 +26,7 @@ import torch
 
 from .. import _native as N
 from .mxfp8 import _QUANT_DT as DTYPES
-from .mxfp8 import _plain_cuda
+from .mxfp8 import _bits, _plain_cuda
 
 BLOCK = 128
 BLOCKS = {"row": (1, BLOCK), "col": (BLOCK, 1), "tile": (BLOCK, BLOCK)}
@@ -187,9 +187,9 @@ def _torch_quantize(x: torch.Tensor, block: str) -> Quantized:
     r, c = _scale_shape(rows, cols, block)
     m, e = torch.frexp(mag.reshape(r, br, c, bc).amax((1, 3)) if x.numel() else mag.new_zeros(r, c))
     e = torch.where(m > 0.875, e - 8, e - 9).clamp(min=-126)      # 448 = 0.875 * 2 ** 9
-    scale = torch.where(m > 0, ((e + 127) << 23).view(torch.float32), torch.ones_like(m))
+    scale = torch.where(m > 0, _bits((e + 127) << 23, torch.float32), torch.ones_like(m))
     q = torch.where(finite, x / _spread(scale, rows, cols, block), torch.full_like(x, float("nan"))).to(torch.float8_e4m3fn)
-    data = _new_payload(rows, cols, x).copy_(q.view(torch.uint8))
+    data = _new_payload(rows, cols, x).copy_(_bits(q, torch.uint8))
     return data, (scale.t().contiguous().t() if block == "row" else scale)
 
 
@@ -205,7 +205,7 @@ def dequantize_fp8(data: torch.Tensor, scale: torch.Tensor, block: str = "row", 
     _check_scale(scale, _scale_shape(rows, cols, block), data, "scale")
     if not _native(data, scale):
         top = torch.finfo(dtype).max
-        return (data.view(torch.float8_e4m3fn).float() * _spread(scale, rows, cols, block)).clamp(-top, top).to(dtype)
+        return (_bits(data, torch.float8_e4m3fn).float() * _spread(scale, rows, cols, block)).clamp(-top, top).to(dtype)
     out = data.new_empty((rows, cols), dtype=dtype)
     if out.numel():
         data, pitch = _payload(data, "data", vectors=True)

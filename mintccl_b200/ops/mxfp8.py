@@ -32,6 +32,28 @@ def scale_to_float(scale: torch.Tensor) -> torch.Tensor:
     return torch.pow(2.0, scale.float() - 127.0)
 
 
+class _Bits(torch.autograd.Function):
+    """``t.view(dtype)`` for types of one size, which vmap has no rule for."""
+    @staticmethod
+    def forward(t, dtype):
+        return t.view(dtype)
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        ctx.mark_non_differentiable(output)
+
+    @staticmethod
+    def vmap(info, in_dims, t, dtype):
+        return _Bits.apply(t, dtype), in_dims[0]
+
+
+def _bits(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """The bits of ``t`` as ``dtype``, under vmap too."""
+    if torch.compiler.is_compiling() or not torch._C._functorch.is_batchedtensor(t):
+        return t.view(dtype)
+    return _Bits.apply(t, dtype)
+
+
 def _is_plain(t: torch.Tensor) -> bool:
     """Whether ``t`` stands for its own memory: not a subclass, nothing that transforms it (vmap, functionalisation, a lazy
     zero or negation), and nobody recording or replacing the operations on it (tracing, compilation, a dispatch mode).  All
@@ -86,11 +108,11 @@ def _torch_quantize(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     flat = x.detach().float().reshape(-1, BLOCK)
     scale = scale_for_amax(flat.abs().amax(dim=1))
     q = (flat / scale_to_float(scale)[:, None]).to(torch.float8_e4m3fn)
-    return q.view(torch.uint8).reshape(-1), scale
+    return _bits(q, torch.uint8).reshape(-1), scale
 
 
 def dequantize_mxfp8(data: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
-    return (data.view(torch.float8_e4m3fn).float().reshape(-1, BLOCK) * scale_to_float(scale)[:, None]).reshape(-1)
+    return (_bits(data, torch.float8_e4m3fn).float().reshape(-1, BLOCK) * scale_to_float(scale)[:, None]).reshape(-1)
 
 
 def _lists(comm, t):

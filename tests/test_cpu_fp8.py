@@ -312,3 +312,36 @@ def test_a_wait_that_ran_out_is_reported(monkeypatch):
                 fp8.check()
         else:
             fp8.check()
+
+
+@pytest.mark.parametrize("block", BLOCKS)
+def test_encoding_under_vmap(block):
+    """Batched by torch: the bytes and values of the matrices one by one."""
+    xs = torch.stack([values((3, 260), torch.float32, seed=i) for i in range(4)]).view(2, 2, 3, 260)
+    enc = lambda t: fp8.quantize_fp8(t, block)                                          # noqa: E731
+    dec = lambda d, s: fp8.dequantize_fp8(d, s, block, torch.bfloat16)                  # noqa: E731
+    data, scale = torch.vmap(torch.vmap(enc))(xs)
+    back = torch.vmap(torch.vmap(dec))(data, scale)
+    for i in range(2):
+        for j in range(2):
+            d, s = enc(xs[i, j])
+            assert torch.equal(data[i, j], d) and torch.equal(scale[i, j], s)
+            assert torch.equal(back[i, j].nan_to_num(), dec(d, s).nan_to_num())
+    data, scale = torch.vmap(enc, in_dims=2)(xs[0].transpose(0, 2))
+    for i in range(2):
+        assert torch.equal(data[i], enc(xs[0, i].t())[0])
+
+
+def test_activations_and_their_gradients_under_vmap():
+    g = torch.Generator().manual_seed(6)
+    gate, up, dy = torch.randn(3, 5, 4, 200, generator=g)
+
+    def both(a, b, d):
+        y, saved = c8.swiglu8_forward(a, b)
+        one = c8.silu8_forward(a)[1]
+        return y, *c8.swiglu8_backward(saved, d), c8.silu8_backward(one, d), c8.save8(a).restore()
+
+    got = torch.vmap(both)(gate, up, dy)
+    for i in range(5):
+        for a, b in zip(got, both(gate[i], up[i], dy[i])):
+            torch.testing.assert_close(a[i], b, rtol=2.0 ** -22, atol=2.0 ** -24)      # fp32 exponentials may differ with the layout

@@ -173,3 +173,12 @@ def test_gemm_refuses_tensors_on_the_cpu(monkeypatch):
     d, s, w = torch.zeros(128, 128, dtype=torch.uint8), torch.zeros(128, 4, dtype=torch.uint8), torch.zeros(256, 128, dtype=torch.uint8)
     with pytest.raises(ValueError, match="CUDA"):
         mx.gemm_mxfp8(d, s, w, torch.zeros(256, 4, dtype=torch.uint8))
+
+
+def test_encoding_and_decoding_under_vmap():
+    x = torch.randn(3, 256, generator=torch.Generator().manual_seed(7))
+    data, scale = torch.vmap(mx.quantize_mxfp8)(x)
+    back = torch.vmap(mx.dequantize_mxfp8)(data, scale)
+    for i in range(3):
+        d, s = mx.quantize_mxfp8(x[i])
+        assert torch.equal(data[i], d) and torch.equal(scale[i], s) and torch.equal(back[i], mx.dequantize_mxfp8(d, s))

@@ -746,3 +746,13 @@ def test_layer_with_a_weight_whose_scales_have_any_value():
     check_product(dx, trip(dy, "row"), w64)
     check_product(dw, trip(dy, "col").t(), trip(x, "tile"))
     fp8.check()
+
+
+def test_encoding_under_vmap_takes_the_torch_path():
+    x = torch.randn(3, 40, 300, device="cuda")
+    for block in fp8.BLOCKS:
+        data, scale = torch.vmap(lambda t: fp8.quantize_fp8(t, block))(x)
+        back = torch.vmap(lambda d, s: fp8.dequantize_fp8(d, s, block))(data, scale)
+        for i in range(3):
+            same_encoding((data[i], scale[i]), x[i], block)
+            assert torch.equal(back[i], fp8.dequantize_fp8(data[i], scale[i], block))
