@@ -756,3 +756,42 @@ def test_encoding_under_vmap_takes_the_torch_path():
         for i in range(3):
             same_encoding((data[i], scale[i]), x[i], block)
             assert torch.equal(back[i], fp8.dequantize_fp8(data[i], scale[i], block))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("given", [False, True], ids=["weight", "encoded_weight"])
+def test_large_layer_and_its_gradients(given, dtype):
+    """All three products on pairs, with scales that the tensor core applies; ragged sizes, rows of a wider tensor."""
+    T, K, Nn = 2050, 2300, 1930
+    g = torch.Generator(device="cuda").manual_seed(12)
+    x = torch.randn(T, K + 4, generator=g, device="cuda").to(dtype)[:, 4:].requires_grad_(True)
+    w = (torch.randn(Nn, K, generator=g, device="cuda") * 0.05 * torch.exp(torch.randn(K, generator=g, device="cuda"))).to(dtype).requires_grad_(True)
+    dy = torch.randn(T, Nn, generator=g, device="cuda").to(dtype)
+    y = fp8.linear_fp8(x, w, fp8.quantize_fp8(w, "tile") if given else None)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    check_product_pow2(y.detach(), trip(x, "row"), trip(w, "tile").t())
+    check_product_pow2(dx, trip(dy, "row"), trip(w, "tile"))
+    check_product_pow2(dw, trip(dy, "col").t(), trip(x, "tile"))
+    fp8.check()
+
+
+@pytest.mark.parametrize("shape", [(33, 300, 130), (2050, 1500, 1600)], ids=["small", "pairs"])
+def test_layer_takes_gradients_of_any_layout(shape):
+    """Expanded along either dimension or both, turned, and every other one of a wider tensor: as contiguous ones."""
+    T, K, Nn = shape
+    g = torch.Generator(device="cuda").manual_seed(13)
+    x = torch.randn(T, K, generator=g, device="cuda", dtype=torch.bfloat16).requires_grad_(True)
+    w = torch.randn(Nn, K, generator=g, device="cuda", dtype=torch.bfloat16).requires_grad_(True)
+    y = fp8.linear_fp8(x, w)
+    wide = torch.randn(T + Nn, 2 * (T + Nn), generator=g, device="cuda", dtype=torch.bfloat16)
+    for dy in (wide[:1, :1].expand(T, Nn), wide[:1, :Nn].expand(T, Nn), wide[:T, :1].expand(T, Nn), wide[:Nn, :T].t(),
+               wide[:T, :2 * Nn:2], wide[1:T + 1, 3:Nn + 3]):
+        got = torch.autograd.grad(y, (x, w), dy, retain_graph=True)
+        want = torch.autograd.grad(y, (x, w), dy.contiguous().clone(), retain_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    got = torch.autograd.grad(y.sum(), (x, w), retain_graph=True)
+    want = torch.autograd.grad(y, (x, w), torch.ones_like(y), retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    with pytest.raises(ValueError, match="plain CUDA tensor"):
+        torch.autograd.grad(y, (x, w), torch.ones(3, T, Nn, device="cuda", dtype=torch.bfloat16), is_grads_batched=True)
+    fp8.check()
