@@ -321,14 +321,14 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_fp8_kernel(const __grid_cons
           const bool fresh = !POW2 || kb == 0, done = !POW2 || kb + 1 == kblocks;
           // both probes in flight at once: each takes some 230 cycles beside the tensor core's own shared-memory traffic
           const bool drained = !fresh || mbar_test(&ctl->acc_empty[b], bph ^ 1),
-                     loaded = PAIR ? mbar_test_cluster(&ctl->full[s], ph) : mbar_test(&ctl->full[s], ph);
+                     loaded = POW2 ? mbar_test_cluster(&ctl->full[s], ph) : mbar_test(&ctl->full[s], ph);
           if (!__all_sync(0xffffffffu, drained && loaded) &&
               ((fresh && !wait_bar_warp(&ctl->acc_empty[b], bph ^ 1, abort_flag, a.timeout_ns)) ||
-               !wait_bar_warp<PAIR>(&ctl->full[s], ph, abort_flag, a.timeout_ns))) {
+               !wait_bar_warp<POW2>(&ctl->full[s], ph, abort_flag, a.timeout_ns))) {
             ok = false;
             break;
           }
-          if (PAIR) fence_acquire_cluster_smem();
+          if (POW2) fence_acquire_cluster_smem();   // scales that threads of both CTAs have written
           tc_fence_after();
           const uint64_t da = TA ? make_smem_desc_mn_sw128(sA + s * A_BYTES, 128 * BK) : make_smem_desc_sw128(sA + s * A_BYTES);
           const uint64_t db = !TB          ? make_smem_desc_sw128(sB + s * B_BYTES)
@@ -427,7 +427,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_fp8_kernel(const __grid_cons
             }
             __syncwarp();
             if (lane == 0) {
-              if (PAIR) mbar_arrive_cluster_release(full_leader + s * 8);
+              if (POW2) mbar_arrive_cluster_release(full_leader + s * 8);
+              else if (PAIR) mbar_arrive_cluster(full_leader + s * 8);
               else mbar_arrive(&ctl->full[s]);
             }
             if constexpr (!POW2) {
