@@ -227,7 +227,7 @@ int mt_gemm_fp8(void* stream, const void* A, int64_t lda, const void* sa, int64_
   return gemm(stream, A, lda, sa, sa_m, sa_k, B, ldb, sb, sb_n, sb_k, C, ldc, dtype, M, N, K, ta, tb, nctas, false);
 }
 
-int mt_fp8_packed(void* stream, int op, const int64_t* v) {
+static int packed(void* stream, int op, const int64_t* v) {
   if (!v) return fail("no arguments");
   auto p = [&](int i) { return (void*)(uintptr_t)v[i]; };
   switch (op) {
@@ -263,6 +263,10 @@ int mt_fp8_packed(void* stream, int op, const int64_t* v) {
     }
     default: return fail("unknown operation");
   }
+}
+
+int mt_fp8_packed(void* stream, int op, const int64_t* v) {
+  return guarded([&]() -> int { return packed(stream, op, v); });
 }
 
 int mt_gemm_fp8_error(void) {

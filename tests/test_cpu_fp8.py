@@ -345,3 +345,12 @@ def test_activations_and_their_gradients_under_vmap():
     for i in range(5):
         for a, b in zip(got, both(gate[i], up[i], dy[i])):
             torch.testing.assert_close(a[i], b, rtol=2.0 ** -22, atol=2.0 ** -24)      # fp32 exponentials may differ with the layout
+
+
+def test_packed_calls_report_what_they_cannot_run():
+    import ctypes
+    from mintccl_b200 import _native as N
+    for op, args in ((99, b"\0" * 64), (-1, b"\0" * 64), (fp8.QUANTIZE, b"\0" * 96), (fp8.GEMM, b"\0" * 160), (fp8.LINEAR_FORWARD, b"\0" * 160),
+                     (fp8.LINEAR_BACKWARD, b"\0" * 168), (fp8.GEMM, None)):
+        assert N.lib().mt_fp8_packed(None, op, args and ctypes.create_string_buffer(args, len(args)).raw) < 0, op
+        assert N.last_error()
