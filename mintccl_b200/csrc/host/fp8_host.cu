@@ -50,7 +50,7 @@ int sms_here() {
 
 // Columns of a tile of 256 rows where the tensor core applies the scales.  In 10 ns: a wave of 256 columns takes 35 a block of
 // 128 along K and 300 beside, and the last one 150 until its only accumulator is stored; a wave of 128 columns 22 and 136.
-// Measured (us, 256 / 128 columns): 8192 x 1792 x 4096 51.0 / 56.1, 8192 x 4096 x 4096 99.8 / 116.0, 8192 x 4096 x 1792 50.5 /
+// Measured (us, 256 / 128 columns, when the rule was made): 8192 x 1792 x 4096 51.0 / 56.1, 8192 x 4096 x 4096 99.8 / 116.0, 8192 x 4096 x 1792 50.5 /
 // 59.2, 1792 x 4096 x 8192 51.0 / 61.0, 1024 x 4096 x 4096 16.8 / 19.2, 8192 x 512 x 8192 37.7 / 45.4, 2048 x 2048 x 2048
 // 14.1 / 13.2, 1024 x 14336 x 512 21.0 / 20.3.
 int pow2_columns(int64_t row_tiles, int64_t N, int64_t blocks, int64_t clusters) {

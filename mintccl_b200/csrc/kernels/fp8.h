@@ -58,8 +58,9 @@ struct Fp8GemmArgs {
   int32_t vec_out;                  // rows of C start on 16-byte boundaries
   uint64_t timeout_ns;
 };
-// bn: columns of a tile, 128, or 256 with pair and pow2.  pair: 256 rows each, on CTA pairs (nctas even).  Else 128 rows each; split (1, 2, 4 or 8): the
-// CTAs that share a tile's blocks along K, at most as many as there are blocks; nctas = split * tiles if it is not 1.
+// bn: columns of a tile, 128, or 256 with pair and pow2.  pair: 256 rows each, on CTA pairs (nctas even).  Else 128 rows
+// each; split (1, 2, 4 or 8): the CTAs that share a tile's blocks along K, at most as many as there are blocks; nctas =
+// split * tiles if it is not 1.
 // pow2: all scales are powers of two (looked at with pair only).
 cudaError_t launch_fp8_gemm(int bn, bool pair, bool pow2, int split, bool ta, bool tb, const Fp8GemmArgs& a, int nctas, cudaStream_t s);
 // *expired = 1 if a wait of the product expired on the current device since the last call (waits for the device).

@@ -71,7 +71,7 @@ __device__ __forceinline__ F2 sigmoid2(float x0, float x1) {
 // Multiplications go two to an instruction (29.7, 48, 29.6 and 53 one by one): the rest is some 12 an element.  U: blocks a
 // thread has in flight; with one the ungated forms took 36 and 34, with two the gated ones 53 and 62.
 // Four CTAs an SM for 16-bit types; fp32 ones have twice the words in flight and spill under that limit (8192 x 1792, gated
-// forward 38, without it 33.5).
+// forward 38, without it 33.5).  Gated and off the vector grid 16-bit ones spill 20 - 44 bytes a thread too (3000 x 4095 39.7).
 template <class T, int VEC, bool GATED, int U>
 __global__ void __launch_bounds__(kThreads, sizeof(typename T::elem) == 2 ? 4 : 0) fp8_act_fwd_kernel(Fp8ActArgs a, RowGrid grid) {
   using E = typename T::elem;

@@ -42,9 +42,11 @@ __global__ void __launch_bounds__(kThreads) fp8_row_kernel(Fp8QuantArgs a, RowGr
 
 // ---- any of the three from one read: a CTA holds a tile of 128 x 128 in registers, a thread 4 rows (32 apart) of 16
 // adjacent columns.  Largest magnitudes are taken on the bit patterns, two to a word; tiles with values that are not finite
-// look at them again.  8192 x 4096 bf16, us: tiles 17.3 (5.8 TB/s), column blocks 18.9, row blocks and tiles from one read 29 (4.6),
-// row and column blocks 32 (4.2); one after the other these two take 35 and 36.5, with the input from the L2 the second time.
-// The 125 registers that two encodings of the same words take leave two CTAs an SM; three spill (50 - 60 us).
+// look at them again.  8192 x 4096 bf16, us: tiles 17.2 (5.9 TB/s), column blocks 18.7, row blocks and tiles from one read 29.6 (4.5),
+// row and column blocks 31.6 (4.2), tiles and column blocks 28.1, all three 36.7; row blocks and then tiles take 34.5, or column
+// blocks 36.1, with the input from the L2 the second time.  The 120 - 128 registers of forms with row blocks leave two CTAs
+// an SM; with three they spill (50 - 60 us).  Tiles and column blocks are under the limit of three for 16-bit types and spill
+// 84 - 96 bytes a thread there; off the vector grid, where shared memory takes part, every form with two encodings does.
 template <class T, int VEC, bool ROW, bool COL, bool TILE>
 __global__ void __launch_bounds__(kThreads, sizeof(typename T::elem) == 2 && !ROW ? 3 : 2) fp8_tile_kernel(Fp8QuantArgs a, uint32_t nct) {
   constexpr int kE = (int)sizeof(typename T::elem);
@@ -61,7 +63,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(typename T::elem) == 2 && !RO
   // rows of this thread that exist, of four; where the first is in a payload, and the distance to the next
   const int64_t r0 = (int64_t)rt * 128 + g, q0 = r0 * a.ldq + c0, qstep = 32 * a.ldq;
   const int live = (int)min((int64_t)4, max((int64_t)0, (a.rows - r0 + 31) >> 5));
-  const bool put = n > 0;   // a row's padding to 16 bytes is zeros; what lies behind it, up to the next row, is not this matrix's
+  const bool put = n > 0;   // a row's padding to 16 bytes is zeros; what lies between that and the next row is not ours
   Span16<T, VEC> in[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i)

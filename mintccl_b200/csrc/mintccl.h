@@ -156,8 +156,8 @@ int mt_mxfp8_quantize(void* stream, int dtype, const void* x, void* data, void* 
 int mt_mxfp8_tile_scales(void* stream, const void* in, void* out, uint64_t rows, uint64_t kb);
 
 // ---- e4m3 with one fp32 scale per block of 128 (host/fp8_host.cu), on the current device -------------------------------
-// Payload rows are ldq bytes apart (a multiple of 16, at least cols; padding up to the next 16 is written as zeros) and start on
-// 16-byte boundaries.  dtype: 0 fp32, 1 fp16, 2 bf16.  ld*: elements between rows.
+// Payload rows are ldq bytes apart (a multiple of 16, at least cols; padding up to the next 16 is written as zeros and may be
+// read, what lies behind it is neither) and start on 16-byte boundaries.  dtype: 0 fp32, 1 fp16, 2 bf16.  ld*: elements between rows.
 // Encodings of x [rows, cols]; any of the three may be null.  row_scale [ceil(cols / 128)][rows] (of blocks 1 x 128),
 // col_scale [ceil(rows / 128)][cols] (128 x 1), tile_scale [ceil(rows / 128)][ceil(cols / 128)].
 int mt_fp8_quantize(void* stream, int dtype, const void* x, int64_t ldx, int64_t rows, int64_t cols, int64_t ldq,
@@ -178,9 +178,9 @@ int mt_fp8_act_backward(void* stream, int dtype, int64_t ldq, const void* h_data
 int mt_gemm_fp8(void* stream, const void* A, int64_t lda, const void* sa, int64_t sa_m, int64_t sa_k, const void* B, int64_t ldb,
                 const void* sb, int64_t sb_n, int64_t sb_k, void* C, int64_t ldc, int dtype, int64_t M, int64_t N, int64_t K,
                 int ta, int tb, int nctas);
-// The functions above with their arguments after `stream` as 64-bit integers (MT_FP8_GEMM has one more: all scales are
-// powers of two, and what is not counts as NaN; ctypes takes 3 us to convert twenty
-// arguments one by one), and the two passes of a linear layer, each of them all of its kernels in one call.
+// The functions above with their arguments after `stream` as 64-bit integers (ctypes takes 3 us to convert twenty one by one),
+// and the two passes of a linear layer, each of them all of its kernels in one call.  MT_FP8_GEMM and the passes have one more,
+// power_of_two: all scales are, and what is not counts as NaN.
 //   MT_FP8_LINEAR_FORWARD   dtype, x, ldx, T, K, w_dtype, w (0: encoded already), ldw, N, xr_data, xr_scale, xt_data, xt_scale
 //                           (both 0: not wanted), w_data, ldwq, w_scale, w_srow, w_scol, y, power_of_two
 //       payloads of x are ceil16(K) bytes a row, xr and xt its row blocks and tiles; w's tiles are written if w is given;

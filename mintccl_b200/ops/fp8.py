@@ -225,9 +225,11 @@ def gemm_fp8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: t
     * ``tb``: ``a [M, K] @ b [K, N]``: the gradient of its input; ``a`` in row blocks, ``b`` in tiles;
     * ``ta`` and ``tb``: ``a[K, M].T @ b [K, N]``: the gradient of its weight; ``a`` in column blocks, ``b`` in tiles.
 
-    Sums are fp32, the product of two blocks' scales has to be in that range too, with one rounding to ``dtype`` (fp32, fp16 or bf16; that of ``out`` where it is given) at the end.
-    ``power_of_two``: the caller's word that every scale is one (``quantize_fp8`` makes no others), which large products are
-    faster for, the tensor cores then apply them; a scale that is not may make what it belongs to NaN."""
+    Sums are fp32, and the product of two blocks' scales has to be in that range too, with one rounding to ``dtype`` (fp32,
+    fp16 or bf16; that of ``out`` where it is given) at the end.  ``power_of_two``: the caller's word that every scale is one
+    (``quantize_fp8`` makes no others), which large products are faster for, the tensor cores then apply them; a scale that is
+    not may make what it belongs to NaN.  There are no torch expressions behind the products: under a dispatch mode (a flop
+    counter, selective checkpointing) and for tensors that do not stand for their own memory they raise ``ValueError``."""
     if ta and not tb:
         raise ValueError("gemm_fp8: ta goes with tb")
     if not _native(a, a_scale, b, b_scale):
